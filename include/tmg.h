@@ -229,6 +229,87 @@ int tmg_quantize_i8(const uint16_t *w_dev, uint32_t rows, uint32_t in, int8_t *q
                     void *stream);
 
 /* ---------------------------------------------------------------------- */
+/* Kernel level: a KV cache in 4 bits.  No counterpart in the reference,    */
+/* whose KvCache holds f32 (src/model.rs:250-332).                          */
+/* ---------------------------------------------------------------------- */
+
+/* Keys and values as 4-bit floats (e2m1: magnitudes 0, 0.5, 1, 1.5, 2, 3, 4,
+ * 6 and a sign) in groups of 32 consecutive dimensions of a head (16 where
+ * the head has 16) that share a power of two s: the smallest with max|x| <=
+ * 7 s, within [2^-100, 2^125], stored as the byte log2(s) + 127.  A code is
+ * x / s rounded to the nearest magnitude, halves to the even code, magnitudes
+ * above 6 to 6.  A group that holds an infinity or a NaN has the byte 255 and
+ * reads back as NaN.
+ *
+ * A sequence's cache of `cap` positions is a slab of tmg_kv4_bytes(cap, nkv,
+ * hd) DEVICE bytes, four planes one after the other: key codes
+ * [nkv][cap][hd / 2] (the even dimension of a pair in the low half byte),
+ * value codes, key scale bytes [nkv][cap][max(1, hd / 32)], value scale
+ * bytes.  Its contents need no initialization: only rows that were written
+ * are ever used.
+ *
+ * f32 rows of a batch are numbered b * rows + t (row t of sequence b),
+ * `*_stride` floats apart (0: no gap between rows; otherwise a multiple of
+ * 4), and 16-byte aligned.  Row t is position pos_b + t, where pos_b is
+ * pos_dev[b], read by the kernels (a DEVICE array of n_seq int32), or `pos`
+ * for every sequence when pos_dev is NULL.  Rows past the capacity by `pos`
+ * are TMG_E_CAPACITY; a sequence whose pos_dev entry is negative, or for
+ * which pos_b + rows passes cap, takes no part in the call: nothing of it is
+ * written, and its output rows are zeros.  rows == 0 or n_seq == 0: nothing
+ * to do.
+ *
+ * All calls enqueue kernels on `stream` (NULL: the current device's default
+ * stream), allocate nothing, and may be captured into a graph.  They use the
+ * stream's device, which must hold the cache and every other pointer. */
+typedef struct tmg_kv4 {
+    void *data;        /* DEVICE, 16-byte aligned: sequence b's slab at data + b * seq_stride */
+    size_t seq_stride; /* bytes, a multiple of 16; unused when n_seq is 1 */
+    uint32_t n_seq;    /* <= 65535 */
+    uint32_t cap;      /* positions of a sequence */
+    uint32_t nkv;      /* KV heads */
+    uint32_t hd;       /* head dim: 16, 32, 64, 128 or 256 */
+} tmg_kv4;
+
+/* Bytes of one sequence's slab (a multiple of 16); 0 for an unsupported shape. */
+size_t tmg_kv4_bytes(uint32_t cap, uint32_t nkv, uint32_t hd);
+
+/* Quantizes rows of k and v, [nkv * hd] f32 each, into the cache. */
+int tmg_kv4_write(const tmg_kv4 *kv, const float *k_dev, const float *v_dev, size_t row_stride, uint32_t rows,
+                  const int32_t *pos_dev, uint32_t pos, void *stream);
+
+/* What the rows at positions pos_b .. pos_b + rows - 1 stand for, as f32
+ * (exactly); k_dev or v_dev may be NULL. */
+int tmg_kv4_read(const tmg_kv4 *kv, float *k_dev, float *v_dev, size_t row_stride, uint32_t rows,
+                 const int32_t *pos_dev, uint32_t pos, void *stream);
+
+/* Causal attention over the cache: row t of sequence b, at position pos_b +
+ * t, attends to positions 0 .. pos_b + t; query head h reads KV head h /
+ * (nq / nkv).  With k_new and v_new the rows' keys and values are first
+ * written as tmg_kv4_write does (one call is a decode step's append and
+ * attention); without them the cache holds the rows already.  Computed in f32
+ * or better: the codes are used exactly, the softmax statistics and sums are
+ * f32.  A row whose scores are all -infinity gives zeros. */
+typedef struct tmg_kv4_attn_args {
+    const float *q;    /* DEVICE rows of [nq * hd] */
+    float *out;        /* DEVICE rows of [nq * hd]; must not overlap the inputs */
+    const float *k_new, *v_new; /* DEVICE rows of [nkv * hd] to append first, or both NULL */
+    size_t q_stride, out_stride, new_stride; /* floats between rows; 0: no gap */
+    uint32_t rows;     /* query rows of a sequence */
+    uint32_t nq;       /* query heads, a multiple of nkv, <= 65536 */
+    const int32_t *pos_dev;
+    uint32_t pos;
+    float scale;       /* of the scores; 0: 1 / sqrt(hd) */
+    void *ws;          /* DEVICE workspace, 16-byte aligned, of at least tmg_kv4_attn_workspace's bytes */
+    size_t ws_bytes;
+} tmg_kv4_attn_args;
+int tmg_kv4_attn(const tmg_kv4 *kv, const tmg_kv4_attn_args *args, void *stream);
+
+/* The workspace that `rows` query rows of nq heads need at any positions (it
+ * may be 0).  Calls that can run at the same time need one each; calls in
+ * stream order may share one, captured or not. */
+int tmg_kv4_attn_workspace(const tmg_kv4 *kv, uint32_t rows, uint32_t nq, size_t *bytes);
+
+/* ---------------------------------------------------------------------- */
 /* Measurement entry points.  No counterpart in the reference: they expose  */
 /* the inner loop of generate (src/model.rs:631-656) without the host       */
 /* callback, and per-kernel timing, for benchmarks.                          */

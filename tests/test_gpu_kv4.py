@@ -1,0 +1,488 @@
+"""The 4-bit KV cache's kernels (tmg_kv4_*) against the numpy reference in 64
+bits (kv4ref.py): codes and values exactly, the attention within the bound
+derived there."""
+import numpy as np
+import pytest
+
+import kv4ref as R
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def T():
+    import tinyminigo_amd as T
+    return T
+
+
+@pytest.fixture(scope="module")
+def H():
+    from tinyminigo_amd import hip as H
+    return H
+
+
+class Cache:
+    """n_seq slabs in device memory, every byte 0xFF (marked groups) at first,
+    and what they should hold, in 64 bits."""
+
+    def __init__(self, T, H, cap, nkv, hd, n_seq=1, gap=0):
+        self.T, self.H, self.cap, self.nkv, self.hd, self.n_seq = T, H, cap, nkv, hd, n_seq
+        self.size = T.kv4_bytes(cap, nkv, hd)
+        self.stride = self.size + gap
+        self.buf = H.DeviceBuffer(self.stride * n_seq)
+        self.buf.fill_byte(0xFF)
+        self.kv = T.Kv4(self.buf.addr, cap=cap, nkv=nkv, hd=hd, n_seq=n_seq, seq_stride=self.stride)
+        self.want = np.full((n_seq, 2, nkv, cap, hd), np.nan)
+
+    def expect(self, k, v, pos):
+        """The rows k, v [n_seq][rows][nkv][hd] at each sequence's position."""
+        for b, p in enumerate(pos):
+            if 0 <= p <= self.cap - k.shape[1]:
+                for i, x in enumerate((k, v)):
+                    self.want[b, i, :, p:p + x.shape[1]] = R.stands_for(x[b]).transpose(1, 0, 2)
+
+    def write(self, k, v, pos, dev=None, stride=0, stream=0):
+        """Through tmg_kv4_write; positions on the device when dev is given."""
+        width = self.nkv * self.hd
+        kd, vd = rows_buffer(self.H, k, stride or width), rows_buffer(self.H, v, stride or width)
+        at = {"pos_dev": dev.addr} if dev else {"pos": pos[0]}
+        self.T.kv4_write(self.kv, kd.addr, vd.addr, k.shape[1], row_stride=stride, stream=stream, **at)
+        self.H.synchronize()
+        self.expect(k, v, pos)
+
+    def fill(self, rng, upto, keys=None, values=None):
+        """Random rows [0, upto) of every sequence."""
+        k, v = rows(rng, self, upto), rows(rng, self, upto)
+        if keys is not None:
+            k = keys(k)
+        if values is not None:
+            v = values(v)
+        self.write(k, v, [0] * self.n_seq)
+        return k, v
+
+    def held(self):
+        raw = self.buf.to_array(np.uint8, self.stride * self.n_seq)
+        return np.stack([R.unpack(raw[b * self.stride:b * self.stride + self.size], self.cap, self.nkv, self.hd)
+                         for b in range(self.n_seq)])
+
+    def check(self):
+        np.testing.assert_array_equal(self.held(), self.want)
+
+
+def rows(rng, c, n):
+    x = rng.standard_normal((c.n_seq, n, c.nkv, c.hd)) * np.exp(0.7 * rng.standard_normal((c.n_seq, n, c.nkv, 1)))
+    return x.astype(np.float32)
+
+
+def rows_buffer(H, x, stride, fill=0.0):
+    """Device rows of x [n_seq][rows][..] at the stride."""
+    flat = x.reshape(x.shape[0] * x.shape[1], -1)
+    out = np.full((flat.shape[0], stride), fill, np.float32)
+    out[:, :flat.shape[1]] = flat
+    return H.DeviceBuffer.from_array(out)
+
+
+def ints(H, x):
+    return H.DeviceBuffer.from_array(np.asarray(x, np.int32))
+
+
+def attend(c, q, pos, dev=None, new=None, q_stride=0, out_stride=0, new_stride=0, scale=None, stream=0):
+    """Through tmg_kv4_attn: [n_seq][rows][nq][hd], and what stands around the
+    rows of the output stays as it was."""
+    T, H = c.T, c.H
+    n_seq, n, nq, hd = q.shape
+    width = nq * hd
+    qd = rows_buffer(H, q, q_stride or width)
+    tail = 40
+    out = H.DeviceBuffer.from_array(np.full(n_seq * n * (out_stride or width) + tail, 7.25, np.float32))
+    ws_bytes = T.kv4_attn_workspace(c.kv, n, nq)
+    ws = H.DeviceBuffer(ws_bytes + 64)
+    ws.fill_byte(0xFF)
+    kd = vd = None
+    if new is not None:
+        kd, vd = (rows_buffer(H, x, new_stride or c.nkv * hd) for x in new)
+    at = {"pos_dev": dev.addr} if dev else {"pos": pos[0]}
+    T.kv4_attn(c.kv, qd.addr, out.addr, n, nq, k_dev=kd.addr if kd else 0, v_dev=vd.addr if vd else 0,
+               q_stride=q_stride, out_stride=out_stride, row_stride=new_stride, scale=scale or 0.0, ws_dev=ws.addr,
+               ws_bytes=ws_bytes, stream=stream, **at)
+    H.synchronize()
+    if new is not None:
+        c.expect(new[0], new[1], pos)
+    raw = out.to_array(np.float32, n_seq * n * (out_stride or width) + tail)
+    assert (raw[-tail:] == 7.25).all()
+    assert (ws.to_array(np.uint8, ws_bytes + 64)[-64:] == 255).all()
+    body = raw[:-tail].reshape(n_seq * n, -1)
+    assert (body[:, width:] == 7.25).all()
+    return body[:, :width].reshape(q.shape)
+
+
+def check_attn(c, got, q, pos, scale=None):
+    for b, p in enumerate(pos):
+        if p < 0 or p + q.shape[1] > c.cap:
+            assert (got[b] == 0).all()
+            continue
+        want, tol = R.attend(q[b], c.want[b, 0], c.want[b, 1], p, scale)
+        np.testing.assert_array_equal(np.isnan(got[b]), np.isnan(want))
+        err = np.abs(got[b] - want)
+        with np.errstate(all="ignore"):
+            worst = np.nanmax(err / tol) if np.isfinite(want).any() else 0.0
+        assert worst <= 1.0, f"sequence {b}: {worst:.3g} times the bound"
+
+
+# ---- rows written and read --------------------------------------------------------
+
+HEADS = [(1, 16), (2, 16), (3, 32), (2, 64), (8, 128), (1, 256), (4, 256)]
+
+
+@pytest.mark.parametrize("nkv,hd", HEADS)
+@pytest.mark.parametrize("cap,pos,n", [(1, 0, 1), (7, 2, 5), (65, 0, 65), (300, 17, 100)])
+def test_write_and_read(T, H, nkv, hd, cap, pos, n):
+    rng = np.random.default_rng(cap * 1000 + nkv * 10 + hd)
+    c = Cache(T, H, cap, nkv, hd)
+    k, v = rows(rng, c, n), rows(rng, c, n)
+    c.write(k, v, [pos])
+    c.check()  # the rows, and nothing else
+    width = nkv * hd
+    kd, vd = (H.DeviceBuffer.from_array(np.full(n * width + 16, 3.5, np.float32)) for _ in range(2))
+    T.kv4_read(c.kv, kd.addr, vd.addr, n, pos=pos)
+    H.synchronize()
+    for d, x in ((kd, k), (vd, v)):
+        got = d.to_array(np.float32, n * width + 16)
+        np.testing.assert_array_equal(got[:-16].reshape(1, n, nkv, hd), R.stands_for(x).astype(np.float32))
+        assert (got[-16:] == 3.5).all()
+
+
+def test_write_rounds_and_scales_by_the_definition(T, H):
+    """Every threshold and its neighbours at many scales, both signs, maxima
+    around 7 times a power of two, the ends of the scale's range, zeros,
+    subnormals, infinities and NaN."""
+    rng = np.random.default_rng(5)
+    th = np.array([0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 6, 7], np.float32)
+    near = np.concatenate([th, np.nextafter(th, np.float32(np.inf)), np.nextafter(th, np.float32(-np.inf))])
+    out = []
+    for e in [-149, -140, -126, -110, -103, -102, -101, -100, -99, -64, -20, -1, 0, 1, 7, 40, 100, 119, 122, 124, 125, 126]:
+        for top in (3.5, 3.75, 4.0, 5.0, 6.0, 6.9999995, 7.0, 7.0000005, 7.5, 7.9999995):
+            g = rng.choice(near, 32) * rng.choice([-1, 1], 32)
+            g[rng.integers(32)] = top
+            with np.errstate(all="ignore"):
+                out.append(np.clip(g.astype(np.float64) * 2.0 ** e, -3.4028234e38, 3.4028234e38).astype(np.float32))
+    for bad in (np.inf, -np.inf, np.nan):
+        g = rng.standard_normal(32).astype(np.float32)
+        g[rng.integers(32)] = bad
+        out.append(g)
+    out.append(np.zeros(32, np.float32))
+    out.append(-np.zeros(32, np.float32))
+    out += [np.zeros(32, np.float32)] * (-len(out) % 8)
+    k = np.stack(out).reshape(1, -1, 2, 128)
+    c = Cache(T, H, k.shape[1] + 1, 2, 128)
+    c.write(k, k[:, ::-1].copy(), [1])
+    c.check()
+
+
+@pytest.mark.parametrize("hd", [16, 128])
+def test_write_batch_by_device_positions(T, H, hd):
+    """Idle slots, rows that would pass the capacity and the sequences' gaps
+    stay as they were; strided rows."""
+    rng = np.random.default_rng(hd)
+    c = Cache(T, H, 40, 2, hd, n_seq=6, gap=48)
+    pos = [3, -1, 36, 37, 0, -2147483648]
+    k, v = rows(rng, c, 4), rows(rng, c, 4)
+    c.write(k, v, pos, dev=ints(H, pos), stride=2 * hd + 12)
+    c.check()
+    raw = c.buf.to_array(np.uint8, c.stride * 6).reshape(6, -1)
+    assert (raw[:, c.size:] == 255).all() and (raw[1] == 255).all() and (raw[3] == 255).all()
+    # read: zeros for the sequences that take no part, gaps left
+    stride = 2 * hd + 4
+    kd = H.DeviceBuffer.from_array(np.full((24, stride), 9.0, np.float32))
+    T.kv4_read(c.kv, kd.addr, 0, 4, pos_dev=ints(H, pos).addr, row_stride=stride)
+    H.synchronize()
+    got = kd.to_array(np.float32, 24 * stride).reshape(6, 4, stride)
+    assert (got[..., 2 * hd:] == 9.0).all()
+    want = R.stands_for(k).reshape(6, 4, -1)
+    for b, p in enumerate(pos):
+        np.testing.assert_array_equal(got[b, :, :2 * hd], want[b] if p in (3, 36, 0) else np.zeros((4, 2 * hd)))
+
+
+# ---- attention ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("ctx", [1, 2, 15, 16, 17, 31, 32, 33, 127, 128, 129, 257, 640, 1111])
+def test_attn_single_token(T, H, ctx):
+    rng = np.random.default_rng(ctx)
+    c = Cache(T, H, 1200, 2, 128)
+    c.fill(rng, ctx)
+    q = rng.standard_normal((1, 1, 4, 128)).astype(np.float32)
+    check_attn(c, attend(c, q, [ctx - 1]), q, [ctx - 1])
+
+
+@pytest.mark.parametrize("nkv,hd", HEADS)
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 8, 20])
+def test_attn_head_layouts(T, H, nkv, hd, group):
+    rng = np.random.default_rng(nkv * 100 + hd + group)
+    c = Cache(T, H, 300, nkv, hd)
+    c.fill(rng, 300)
+    for n in (1, 7):
+        q = rng.standard_normal((1, n, nkv * group, hd)).astype(np.float32)
+        pos = [int(rng.integers(0, 300 - n))]
+        check_attn(c, attend(c, q, pos), q, pos)
+
+
+@pytest.mark.parametrize("hd,group", [(16, 2), (64, 4), (128, 2), (128, 4), (128, 1), (256, 2)])
+@pytest.mark.parametrize("n,pos", [(2, 0), (8, 5), (17, 0), (33, 31), (64, 64), (45, 300), (130, 0), (200, 77)])
+def test_attn_pieces(T, H, hd, group, n, pos):
+    rng = np.random.default_rng(n * 7 + hd + group)
+    c = Cache(T, H, pos + n + 3, 2, hd)
+    c.fill(rng, pos + n)
+    q = rng.standard_normal((1, n, 2 * group, hd)).astype(np.float32)
+    check_attn(c, attend(c, q, [pos]), q, [pos])
+
+
+@pytest.mark.parametrize("n,pos", [(257, 0), (300, 1000)])
+def test_attn_longer_pieces(T, H, n, pos):
+    rng = np.random.default_rng(n)
+    c = Cache(T, H, pos + n, 1, 128)
+    c.fill(rng, pos + n)
+    q = rng.standard_normal((1, n, 2, 128)).astype(np.float32)
+    check_attn(c, attend(c, q, [pos]), q, [pos])
+
+
+def test_attn_sharp_and_flat_softmax(T, H):
+    """Scores of some hundreds, one dominant key, and equal keys."""
+    rng = np.random.default_rng(9)
+    c = Cache(T, H, 500, 2, 64)
+    c.fill(rng, 500, keys=lambda k: (k * np.where(np.arange(500) % 250 < 125, 8.0, 0.0)[None, :, None, None]).astype(np.float32))
+    q = (6 * rng.standard_normal((1, 3, 8, 64))).astype(np.float32)
+    check_attn(c, attend(c, q, [497]), q, [497])
+    check_attn(c, attend(c, q, [497], scale=1e-3), q, [497], scale=np.float64(np.float32(1e-3)))
+
+
+@pytest.mark.parametrize("n", [1, 5])
+@pytest.mark.parametrize("nkv,hd,group", [(2, 16, 2), (8, 128, 2), (2, 128, 4)])
+def test_attn_batch_by_device_positions(T, H, n, nkv, hd, group):
+    """Ragged positions, an idle slot in the middle and at the end, one past
+    the capacity; strided rows of q and of the output."""
+    rng = np.random.default_rng(n + hd)
+    c = Cache(T, H, 700, nkv, hd, n_seq=7, gap=16)
+    c.fill(rng, 700)
+    pos = [0, 131, -1, 695, 699 if n == 1 else 700, 12, -5]
+    q = rng.standard_normal((7, n, nkv * group, hd)).astype(np.float32)
+    w = nkv * group * hd
+    check_attn(c, attend(c, q, pos, dev=ints(H, pos), q_stride=w + 8, out_stride=w + 20), q, pos)
+
+
+@pytest.mark.parametrize("n", [1, 6, 40])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128, 256])
+def test_attn_appends_rows(T, H, n, hd):
+    """New rows are written, and attended to, in the same call; a run of calls
+    as a session makes them."""
+    rng = np.random.default_rng(n + hd)
+    c = Cache(T, H, 400, 2, hd, n_seq=3)
+    at = [0, 64, 250]
+    c.fill(rng, 250)
+    for step in range(3):
+        pos = [p + step * n for p in at]
+        new = rows(rng, c, n), rows(rng, c, n)
+        q = rng.standard_normal((3, n, 4, hd)).astype(np.float32)
+        got = attend(c, q, pos, dev=ints(H, pos), new=new, new_stride=2 * hd + 4)
+        c.check()
+        check_attn(c, got, q, pos)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_attn_append_idle_slots_write_nothing(T, H, n):
+    rng = np.random.default_rng(n)
+    c = Cache(T, H, 200, 2, 128, n_seq=3)
+    c.fill(rng, 150)
+    pos = [150, -1, 201 - n]
+    q = rng.standard_normal((3, n, 4, 128)).astype(np.float32)
+    got = attend(c, q, pos, dev=ints(H, pos), new=(rows(rng, c, n), rows(rng, c, n)))
+    c.check()
+    check_attn(c, got, q, pos)
+
+
+@pytest.mark.parametrize("hd", [16, 64, 128, 256])
+@pytest.mark.parametrize("n,pos", [(1, 200), (9, 195), (60, 150), (140, 60)])
+def test_attn_not_finite_values(T, H, hd, n, pos):
+    """A group of values with an infinity or a NaN makes its 32 dimensions NaN
+    for the rows that see it, and for no others."""
+    rng = np.random.default_rng(hd + n)
+    c = Cache(T, H, pos + n, 2, hd)
+
+    def spoil(v):
+        v[0, pos + n // 2, 0, hd - 1] = np.inf
+        v[0, pos + n - 1, 1, 0] = np.nan
+        return v
+    c.fill(rng, pos + n, values=spoil)
+    q = rng.standard_normal((1, n, 4, hd)).astype(np.float32)
+    got = attend(c, q, [pos])
+    check_attn(c, got, q, [pos])
+    assert np.isnan(got).any() and (n == 1 or not np.isnan(got[0, 0]).any())
+
+
+@pytest.mark.parametrize("hd", [16, 64, 128, 256])
+@pytest.mark.parametrize("n,pos", [(1, 200), (9, 195), (60, 150), (140, 60)])
+def test_attn_not_finite_keys(T, H, hd, n, pos):
+    """A key with a NaN makes the rows that see it NaN, and no others."""
+    rng = np.random.default_rng(hd + n)
+    c = Cache(T, H, pos + n, 2, hd)
+
+    def spoil(k):
+        k[0, pos + n // 2, 0, 0] = np.nan
+        return k
+    c.fill(rng, pos + n, keys=spoil)
+    q = rng.standard_normal((1, n, 4, hd)).astype(np.float32)
+    got = attend(c, q, [pos])
+    check_attn(c, got, q, [pos])
+    assert np.isnan(got[0, n // 2:, :2]).all() and not np.isnan(got[0, :, 2:]).any()
+
+
+def test_attn_all_keys_not_finite(T, H):
+    """Runs of keys without a single finite score are not left out."""
+    rng = np.random.default_rng(1)
+    c = Cache(T, H, 1000, 1, 64)
+
+    def spoil(k):
+        k[0, 300:700] = np.nan
+        return k
+    c.fill(rng, 1000, keys=spoil)
+    q = rng.standard_normal((1, 1, 2, 64)).astype(np.float32)
+    for p in (299, 300, 999):
+        got = attend(c, q, [p])
+        assert np.isnan(got).all() == (p >= 300)
+        check_attn(c, got, q, [p])
+
+
+def test_attn_not_finite_queries(T, H):
+    """A query row with an infinity or a NaN is NaN; its neighbours are not."""
+    rng = np.random.default_rng(2)
+    c = Cache(T, H, 300, 2, 128)
+    c.fill(rng, 300)
+    q = rng.standard_normal((1, 20, 4, 128)).astype(np.float32)
+    q[0, 3, 1, 77] = np.nan
+    q[0, 11, 2, 0] = np.inf
+    got = attend(c, q, [280])
+    bad = np.isnan(got).all(-1)[0]
+    assert bad[3, 1] and bad[11, 2] and bad.sum() == 2
+    q = np.nan_to_num(q, nan=0.0, posinf=0.0)
+    again = attend(c, q, [280])
+    assert (got[0][~bad] == again[0][~bad]).all()
+    check_attn(c, again, q, [280])
+
+
+def test_attn_large_and_small_magnitudes(T, H):
+    """Values around 2^60 and 2^-60 and in one sequence; scores whose spread
+    is past f32's exponential."""
+    rng = np.random.default_rng(4)
+    c = Cache(T, H, 260, 2, 128)
+    c.fill(rng, 260, values=lambda v: (v * np.exp2(rng.integers(-60, 61, (1, 260, 1, 1)))).astype(np.float32),
+           keys=lambda k: (k * np.exp2(rng.integers(-6, 4, (1, 260, 1, 1)))).astype(np.float32))
+    q = rng.standard_normal((1, 2, 4, 128)).astype(np.float32)
+    check_attn(c, attend(c, q, [258]), q, [258])
+
+
+def test_attn_on_a_stream_and_in_graphs(T, H):
+    """A decode step's append and attention captured by device position and
+    replayed as the position advances, two graphs with one workspace in one
+    stream; every replay against the eager result."""
+    rng = np.random.default_rng(8)
+    c, e = (Cache(T, H, 600, 2, 128, n_seq=2) for _ in range(2))
+    k0, v0 = c.fill(rng, 300)
+    e.write(k0, v0, [0, 0])
+    width, nq = 2 * 128, 4
+    s = H.Stream()
+    kd, vd = H.DeviceBuffer(2 * width * 4), H.DeviceBuffer(2 * width * 4)
+    qd = [H.DeviceBuffer(2 * nq * 128 * 4) for _ in range(2)]
+    out = [H.DeviceBuffer(2 * nq * 128 * 4) for _ in range(2)]
+    pd = ints(H, [0, 0])
+    ws = H.DeviceBuffer(T.kv4_attn_workspace(c.kv, 1, nq))
+    ws.fill_byte(0)
+
+    def step(i):
+        def go(st):
+            T.kv4_attn(c.kv, qd[i].addr, out[i].addr, 1, nq, pos_dev=pd.addr, k_dev=kd.addr, v_dev=vd.addr,
+                       ws_dev=ws.addr, ws_bytes=ws.nbytes, stream=st.addr)
+        return go
+    graphs = [H.Graph(s, step(i)) for i in range(2)]
+    for n in range(4):
+        pos = [300 + n, 17 + n]
+        new = rows(rng, c, 1), rows(rng, c, 1)
+        q = rng.standard_normal((2, 2, 1, nq, 128)).astype(np.float32)
+        for d, x in [(kd, new[0]), (vd, new[1]), (qd[0], q[0]), (qd[1], q[1]), (pd, np.asarray(pos, np.int32))]:
+            H.copy_device(d, H.DeviceBuffer.from_array(x), x.nbytes)
+        for g in graphs:
+            g.launch()
+        s.synchronize()
+        c.expect(new[0], new[1], pos)
+        for i in range(2):
+            got = out[i].to_array(np.float32, q[i].size).reshape(q[i].shape)
+            eager = attend(e, q[i], pos, dev=ints(H, pos), new=new)
+            np.testing.assert_array_equal(got, eager)
+            check_attn(c, got, q[i], pos)
+        c.check()
+
+
+def test_attn_two_streams_at_once(T, H):
+    """Calls with a workspace each overlap on two streams."""
+    rng = np.random.default_rng(12)
+    c = Cache(T, H, 3000, 2, 128)
+    c.fill(rng, 3000)
+    nq, streams = 4, [H.Stream(), H.Stream()]
+    q = rng.standard_normal((8, 1, 1, nq, 128)).astype(np.float32)
+    qd = [H.DeviceBuffer.from_array(x) for x in q]
+    out = [H.DeviceBuffer(nq * 512) for _ in q]
+    ws = [H.DeviceBuffer(T.kv4_attn_workspace(c.kv, 1, nq)) for _ in streams]
+    for w in ws:
+        w.fill_byte(0)
+    for i in range(8):
+        T.kv4_attn(c.kv, qd[i].addr, out[i].addr, 1, nq, pos=2990 + i, ws_dev=ws[i % 2].addr, ws_bytes=ws[i % 2].nbytes,
+                   stream=streams[i % 2].addr)
+    for s in streams:
+        s.synchronize()
+    for i in range(8):
+        check_attn(c, out[i].to_array(np.float32, nq * 128).reshape(q[i].shape), q[i], [2990 + i])
+
+
+def test_attn_is_the_same_every_time(T, H):
+    rng = np.random.default_rng(13)
+    c = Cache(T, H, 2000, 8, 128)
+    c.fill(rng, 2000)
+    for n in (1, 30):
+        q = rng.standard_normal((1, n, 16, 128)).astype(np.float32)
+        first = attend(c, q, [1900])
+        for _ in range(5):
+            np.testing.assert_array_equal(first, attend(c, q, [1900]))
+
+
+def test_offsets_past_32_bits(T, H):
+    """A cache of 2^22 + 64 positions, 4.6 GB: the same 2^16 rows over and
+    over, so that the attention over all of them is the one over a copy."""
+    rng = np.random.default_rng(21)
+    nkv, hd, part, copies = 8, 128, 1 << 16, 64
+    cap = part * copies + 64
+    buf = H.DeviceBuffer(T.kv4_bytes(cap, nkv, hd))
+    kv = T.Kv4(buf.addr, cap=cap, nkv=nkv, hd=hd)
+    k, v = (rng.standard_normal((part, nkv, hd), dtype=np.float32) for _ in range(2))
+    kd, vd = H.DeviceBuffer.from_array(k), H.DeviceBuffer.from_array(v)
+    for i in range(copies):
+        T.kv4_write(kv, kd.addr, vd.addr, part, pos=i * part)
+    H.synchronize()
+    for pos in (0, part * (copies - 1) + 5, part * copies - 3):
+        back = H.DeviceBuffer(3 * nkv * hd * 4)
+        T.kv4_read(kv, 0, back.addr, 3, pos=pos)
+        H.synchronize()
+        np.testing.assert_array_equal(back.to_array(np.float32, 3 * nkv * hd).reshape(3, nkv, hd),
+                                      R.stands_for(v[np.arange(pos, pos + 3) % part]).astype(np.float32))
+    q = rng.standard_normal((1, 1, 16, hd)).astype(np.float32)
+    qd, out = H.DeviceBuffer.from_array(q), H.DeviceBuffer(16 * hd * 4)
+    ws = H.DeviceBuffer(T.kv4_attn_workspace(kv, 1, 16))
+    ws.fill_byte(0)
+    T.kv4_attn(kv, qd.addr, out.addr, 1, 16, pos=part * copies - 1, ws_dev=ws.addr, ws_bytes=ws.nbytes)
+    H.synchronize()
+    got = out.to_array(np.float32, 16 * hd).reshape(16, hd)
+    kk, vv = R.stands_for(k).transpose(1, 0, 2), R.stands_for(v).transpose(1, 0, 2)
+    want, tol = R.attend(q[0], kk, vv, part - 1)
+    # 64 times the weights: the bound's n / 8 grows by as much
+    tol *= (4 + 2 * (16 + part * copies / 8)) / (4 + 2 * (16 + part / 8))
+    assert (np.abs(got - want[0]) <= tol[0]).all()
+    assert np.linalg.norm(got - want[0]) <= 1e-5 * np.linalg.norm(want[0])

@@ -7,12 +7,13 @@ prefill.  This package binds it with ctypes behind the reference's model API.
 """
 from ._lib import TmgError, lib
 from .model import (
-    GenOutput, GenParams, KvCache, Model, ModelConfig, argmax_f32, gemv_bf16, gemv_f32, gemv_i8, generate,
-    generate_batch, prefill_plan, profile_stream, quantize_i8, repack_tmb, stdrng_uniform, synth_model, synth_normal_bf16,
+    GenOutput, GenParams, Kv4, KvCache, Model, ModelConfig, argmax_f32, gemv_bf16, gemv_f32, gemv_i8, generate,
+    generate_batch, kv4_attn, kv4_attn_workspace, kv4_bytes, kv4_read, kv4_write, prefill_plan, profile_stream, quantize_i8, repack_tmb, stdrng_uniform, synth_model, synth_normal_bf16,
     synth_normal_f32, synth_tokens,
 )
 
 __all__ = [
-    "TmgError", "lib", "argmax_f32", "GenOutput", "GenParams", "KvCache", "Model", "ModelConfig", "gemv_bf16", "gemv_f32", "gemv_i8",
-    "generate", "generate_batch", "prefill_plan", "profile_stream", "quantize_i8", "repack_tmb", "stdrng_uniform", "synth_model", "synth_normal_bf16", "synth_normal_f32", "synth_tokens",
+    "TmgError", "lib", "argmax_f32", "GenOutput", "GenParams", "Kv4", "KvCache", "Model", "ModelConfig", "gemv_bf16", "gemv_f32", "gemv_i8",
+    "generate", "generate_batch", "kv4_attn", "kv4_attn_workspace", "kv4_bytes", "kv4_read", "kv4_write",
+    "prefill_plan", "profile_stream", "quantize_i8", "repack_tmb", "stdrng_uniform", "synth_model", "synth_normal_bf16", "synth_normal_f32", "synth_tokens",
 ]

@@ -97,6 +97,18 @@ class tmg_synth_spec(C.Structure):
     ]
 
 
+class tmg_kv4(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("seq_stride", C.c_size_t), ("n_seq", C.c_uint32), ("cap", C.c_uint32),
+                ("nkv", C.c_uint32), ("hd", C.c_uint32)]
+
+
+class tmg_kv4_attn_args(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("k_new", C.c_void_p), ("v_new", C.c_void_p),
+                ("q_stride", C.c_size_t), ("out_stride", C.c_size_t), ("new_stride", C.c_size_t),
+                ("rows", C.c_uint32), ("nq", C.c_uint32), ("pos_dev", C.c_void_p), ("pos", C.c_uint32),
+                ("scale", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
 ON_TOKEN = C.CFUNCTYPE(None, C.c_uint32, C.c_void_p)
 
 P = C.c_void_p
@@ -135,6 +147,11 @@ SIGNATURES = {
     "tmg_stdrng_uniform": (C.c_int, [C.c_uint64, C.c_size_t, PF]),
     "tmg_gemv_i8": (C.c_int, [P, P, P, P, C.c_uint32, C.c_uint32, P]),
     "tmg_quantize_i8": (C.c_int, [P, C.c_uint32, C.c_uint32, P, P, P]),
+    "tmg_kv4_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32]),
+    "tmg_kv4_write": (C.c_int, [C.POINTER(tmg_kv4), P, P, C.c_size_t, C.c_uint32, P, C.c_uint32, P]),
+    "tmg_kv4_read": (C.c_int, [C.POINTER(tmg_kv4), P, P, C.c_size_t, C.c_uint32, P, C.c_uint32, P]),
+    "tmg_kv4_attn": (C.c_int, [C.POINTER(tmg_kv4), C.POINTER(tmg_kv4_attn_args), P]),
+    "tmg_kv4_attn_workspace": (C.c_int, [C.POINTER(tmg_kv4), C.c_uint32, C.c_uint32, C.POINTER(C.c_size_t)]),
     "tmg_decode_greedy": (C.c_int, [P, P, C.c_uint32, C.c_uint32, PU32, PF]),
     "tmg_prefill_plan": (C.c_int, [C.POINTER(tmg_config), C.c_int, C.c_uint32, C.c_uint32, C.POINTER(tmg_plan_record),
                                    C.c_size_t, C.POINTER(C.c_size_t)]),

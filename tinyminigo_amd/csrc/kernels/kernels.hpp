@@ -349,6 +349,80 @@ __host__ __device__ constexpr int attn_chunk(int hd, int group, int nt, int chw)
 // the blocks of its inactive splits.
 constexpr int kSpecSplits = 8;
 
+// ---- 4-bit KV cache -----------------------------------------------------------
+
+// Slabs of one layer's keys and values, one per sequence (the number format
+// and the planes of a slab: kv4.cuh).
+struct Kv4Cache {
+    uint8_t *data;
+    size_t seq_stride;  // bytes from a sequence's slab to the next
+    int n_seq;
+    uint32_t cap;       // positions
+    int nkv, hd;        // hd 16, 32, 64, 128 or 256
+};
+// Scales of a row: one per 32 dimensions, or one.
+__host__ __device__ constexpr int kv4_groups(int hd) { return hd >= 32 ? hd / 32 : 1; }
+// Bytes of a slab, to a multiple of 16: codes and scales of nkv x cap rows.
+__host__ __device__ constexpr size_t kv4_slab_bytes(uint32_t cap, int nkv, int hd) {
+    return ((size_t)nkv * cap * (hd + 2 * kv4_groups(hd)) + 15) / 16 * 16;
+}
+
+// Row t of sequence b is row b * rows + t of the f32 side (row_stride floats
+// apart, [nkv][hd]) and position (pos_dev ? pos_dev[b] : pos) + t of the
+// cache.  A sequence with a negative position, or whose rows would pass the
+// capacity, takes no part: nothing is written; it reads as zeros.
+struct Kv4WriteArgs {
+    Kv4Cache c;
+    const float *k, *v;
+    size_t row_stride;
+    int rows;
+    const int *pos_dev;
+    int pos;
+};
+hipError_t launch_kv4_write(const Kv4WriteArgs &a, hipStream_t s);
+struct Kv4ReadArgs {
+    Kv4Cache c;
+    float *k, *v;  // either may be null
+    size_t row_stride;
+    int rows;
+    const int *pos_dev;
+    int pos;
+};
+hipError_t launch_kv4_read(const Kv4ReadArgs &a, hipStream_t s);
+
+// Row t of sequence b attends to positions 0 .. its own.  A sequence that
+// takes no part (as above) gets zeros.
+struct Kv4AttnArgs {
+    Kv4Cache c;
+    const float *q;  // rows of [nq][hd]
+    size_t q_stride;
+    float *out;  // rows of [nq][hd], or null
+    size_t out_stride;
+    uint16_t *out_hi, *out_lo;  // split-bf16 output (prefill), or null
+    int nq, rows;
+    const int *pos_dev;
+    int pos;
+    float scale;
+    // set by launch_kv4_attn: the column tiles' splits and their partial
+    // states [sequence][tile][KV head][split][part_cols] of hd floats in part
+    // and of (max, sum) in part_ml
+    int nsplit, tile_cols, part_cols;
+    float *part, *part_ml;
+};
+constexpr int kKv4Block = 128;       // positions per block of the splits
+constexpr int kKv4MaxSplits = 64;
+constexpr int kKv4Workgroups = 512;  // two per CU
+struct Kv4Plan {
+    int tile_cols, part_cols;  // columns (query rows x heads of a KV head) of a workgroup, and of its partial states
+    int64_t tiles;             // column tiles of all sequences and KV heads
+    int nsplit;                // workgroups that share a tile's keys
+};
+// The launch for contexts of up to ctx positions.
+Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq, uint32_t ctx);
+// Floats of the partial states, enough for every context of the cache.
+size_t kv4_attn_part_floats(const Kv4Cache &c, int rows, int nq);
+hipError_t launch_kv4_attn(Kv4AttnArgs a, float *ws, hipStream_t s);
+
 // ---- sampling --------------------------------------------------------------
 
 // Largest top_k the device sampler supports, and the per-workgroup slice of

@@ -18,13 +18,14 @@ import weakref
 
 from ._lib import (
     ON_TOKEN, TmgError, check, finalizing, lib, register, tmg_config, tmg_floor_record, tmg_gen_params,
-    tmg_kernel_record, tmg_plan_record, tmg_synth_spec,
+    tmg_kernel_record, tmg_kv4, tmg_kv4_attn_args, tmg_plan_record, tmg_synth_spec,
 )
 
 __all__ = [
     "ModelConfig", "Model", "KvCache", "GenParams", "GenOutput", "generate", "gemv_bf16", "gemv_i8", "quantize_i8", "repack_tmb",
     "argmax_f32", "prefill_plan", "profile_stream",
     "generate_batch",
+    "Kv4", "kv4_bytes", "kv4_write", "kv4_read", "kv4_attn", "kv4_attn_workspace",
     "synth_model", "synth_tokens", "synth_normal_bf16", "synth_normal_f32", "TmgError",
 ]
 
@@ -354,6 +355,51 @@ def quantize_i8(w_dev: int, rows: int, in_: int, q_dev: int, scale_dev: int, str
     """WMat::quantize_i8 (src/tensor.rs:275-293) of BF16 rows on device pointers."""
     check(lib.tmg_quantize_i8(C.c_void_p(w_dev), rows, in_, C.c_void_p(q_dev), C.c_void_p(scale_dev),
                               C.c_void_p(stream)))
+
+
+# -- 4-bit KV cache (no reference counterpart) -----------------------------------
+
+def kv4_bytes(cap: int, nkv: int, hd: int) -> int:
+    """Device bytes of one sequence's 4-bit cache of cap positions
+    (tmg_kv4_bytes); 0 for an unsupported shape."""
+    return lib.tmg_kv4_bytes(cap, nkv, hd)
+
+
+class Kv4:
+    """A 4-bit KV cache in device memory the caller owns (tmg_kv4): n_seq slabs
+    of kv4_bytes(cap, nkv, hd) bytes, seq_stride bytes apart."""
+
+    def __init__(self, data_dev: int, *, cap: int, nkv: int, hd: int, n_seq: int = 1, seq_stride: int = 0):
+        self._c = tmg_kv4(data_dev, seq_stride, n_seq, cap, nkv, hd)
+
+
+def kv4_write(kv: Kv4, k_dev: int, v_dev: int, rows: int, pos: int = 0, pos_dev: int = 0, row_stride: int = 0,
+              stream: int = 0) -> None:
+    """Quantize f32 key and value rows into the cache (tmg_kv4_write)."""
+    check(lib.tmg_kv4_write(C.byref(kv._c), k_dev, v_dev, row_stride, rows, pos_dev, pos, stream))
+
+
+def kv4_read(kv: Kv4, k_dev: int, v_dev: int, rows: int, pos: int = 0, pos_dev: int = 0, row_stride: int = 0,
+             stream: int = 0) -> None:
+    """Read cached rows back as f32 (tmg_kv4_read); k_dev or v_dev may be 0."""
+    check(lib.tmg_kv4_read(C.byref(kv._c), k_dev, v_dev, row_stride, rows, pos_dev, pos, stream))
+
+
+def kv4_attn(kv: Kv4, q_dev: int, out_dev: int, rows: int, nq: int, pos: int = 0, pos_dev: int = 0, k_dev: int = 0,
+             v_dev: int = 0, q_stride: int = 0, out_stride: int = 0, row_stride: int = 0, scale: float = 0.0,
+             ws_dev: int = 0, ws_bytes: int = 0, stream: int = 0) -> None:
+    """Causal attention over the cache, after appending the rows k_dev / v_dev
+    when given (tmg_kv4_attn)."""
+    a = tmg_kv4_attn_args(q_dev, out_dev, k_dev, v_dev, q_stride, out_stride, row_stride, rows, nq, pos_dev, pos, scale,
+                          ws_dev, ws_bytes)
+    check(lib.tmg_kv4_attn(C.byref(kv._c), C.byref(a), stream))
+
+
+def kv4_attn_workspace(kv: Kv4, rows: int, nq: int) -> int:
+    """Workspace bytes of kv4_attn (tmg_kv4_attn_workspace)."""
+    n = C.c_size_t()
+    check(lib.tmg_kv4_attn_workspace(C.byref(kv._c), rows, nq, C.byref(n)))
+    return n.value
 
 
 # -- synthetic inputs ---------------------------------------------------------

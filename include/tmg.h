@@ -265,7 +265,7 @@ typedef struct tmg_kv4 {
     void *data;        /* DEVICE, 16-byte aligned: sequence b's slab at data + b * seq_stride */
     size_t seq_stride; /* bytes, a multiple of 16; unused when n_seq is 1 */
     uint32_t n_seq;    /* <= 65535 */
-    uint32_t cap;      /* positions of a sequence */
+    uint32_t cap;      /* positions of a sequence, <= 2^30 */
     uint32_t nkv;      /* KV heads */
     uint32_t hd;       /* head dim: 16, 32, 64, 128 or 256 */
 } tmg_kv4;
@@ -299,14 +299,16 @@ typedef struct tmg_kv4_attn_args {
     const int32_t *pos_dev;
     uint32_t pos;
     float scale;       /* of the scores; 0: 1 / sqrt(hd) */
-    void *ws;          /* DEVICE workspace, 16-byte aligned, of at least tmg_kv4_attn_workspace's bytes */
+    void *ws;          /* DEVICE workspace, see tmg_kv4_attn_workspace; 16-byte aligned */
     size_t ws_bytes;
 } tmg_kv4_attn_args;
 int tmg_kv4_attn(const tmg_kv4 *kv, const tmg_kv4_attn_args *args, void *stream);
 
 /* The workspace that `rows` query rows of nq heads need at any positions (it
- * may be 0).  Calls that can run at the same time need one each; calls in
- * stream order may share one, captured or not. */
+ * may be 0).  It is to be zeroed once, before its first use; every call
+ * leaves it fit for the next, of whatever shape.  Calls that can run at the
+ * same time need one each; calls in stream order may share one, captured or
+ * not. */
 int tmg_kv4_attn_workspace(const tmg_kv4 *kv, uint32_t rows, uint32_t nq, size_t *bytes);
 
 /* ---------------------------------------------------------------------- */

@@ -98,8 +98,7 @@ def attend(c, q, pos, dev=None, new=None, q_stride=0, out_stride=0, new_stride=0
     tail = 40
     out = H.DeviceBuffer.from_array(np.full(n_seq * n * (out_stride or width) + tail, 7.25, np.float32))
     ws_bytes = T.kv4_attn_workspace(c.kv, n, nq)
-    ws = H.DeviceBuffer(ws_bytes + 64)
-    ws.fill_byte(0xFF)
+    ws = H.DeviceBuffer.from_array(np.concatenate([np.zeros(ws_bytes, np.uint8), np.full(64, 255, np.uint8)]))
     kd = vd = None
     if new is not None:
         kd, vd = (rows_buffer(H, x, new_stride or c.nkv * hd) for x in new)

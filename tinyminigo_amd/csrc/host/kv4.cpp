@@ -53,7 +53,7 @@ int launched(hipError_t e, const char *what) {
 
 bool shape_ok(uint32_t cap, uint32_t nkv, uint32_t hd) {
     const bool head = hd == 16 || hd == 32 || hd == 64 || hd == 128 || hd == 256;
-    return head && nkv >= 1 && nkv <= 32767 && cap >= 1 && cap <= 0x7fffff00u;
+    return head && nkv >= 1 && nkv <= 32767 && cap >= 1 && cap <= 1u << 30;
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -62,7 +62,7 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 int check_cache(const tmg_kv4 *kv, uint32_t rows, const int32_t *pos_dev, uint32_t pos) {
     if (!kv || !kv->data) return set_error(TMG_E_INVALID, "null 4-bit cache");
     if (!shape_ok(kv->cap, kv->nkv, kv->hd))
-        return set_error(TMG_E_INVALID, "a 4-bit cache has 1..2147483392 positions, 1..32767 KV heads and a head_dim of 16, 32, 64, 128 or 256");
+        return set_error(TMG_E_INVALID, "a 4-bit cache has 1..2^30 positions, 1..32767 KV heads and a head_dim of 16, 32, 64, 128 or 256");
     if (!aligned16(kv->data) || kv->seq_stride % 16 != 0)
         return set_error(TMG_E_INVALID, "a 4-bit cache is 16-byte aligned, and so is its sequence stride");
     if (kv->n_seq > 65535) return set_error(TMG_E_INVALID, "at most 65535 sequences");
@@ -130,9 +130,9 @@ namespace {
 int check_heads(const tmg_kv4 *kv, uint32_t rows, uint32_t nq) {
     if (nq == 0 || nq % kv->nkv != 0 || nq > 65536)
         return set_error(TMG_E_INVALID, "query heads must be a multiple of the KV heads");
-    // columns, tiles and workgroups stay within 31 bits
+    // columns and workgroups stay within 31 bits
     const uint64_t ncol = (uint64_t)rows * (nq / kv->nkv);
-    if (ncol > 0x7ffffff0u || (ncol + 15) / 16 * kv->nkv * kv->n_seq > 0x7fffffffu / kKv4MaxSplits)
+    if (ncol > 0x7ffffff0u || (ncol + 15) / 16 * kv->nkv * kv->n_seq > 0x7fffffffu)
         return set_error(TMG_E_INVALID, "too many query rows for one call");
     return TMG_OK;
 }
@@ -145,7 +145,7 @@ extern "C" int tmg_kv4_attn_workspace(const tmg_kv4 *kv, uint32_t rows, uint32_t
     int rc = check_cache(kv, rows, nullptr, 0);
     if (!rc) rc = check_heads(kv, rows, nq);
     if (rc) return rc;
-    *bytes = rows && kv->n_seq ? kv4_attn_part_floats(view(kv), (int)rows, (int)nq) * 4 : 0;
+    *bytes = rows && kv->n_seq ? kv4_attn_ws_bytes(view(kv), (int)rows, (int)nq) : 0;
     return TMG_OK;
 }
 
@@ -165,15 +165,11 @@ extern "C" int tmg_kv4_attn(const tmg_kv4 *kv, const tmg_kv4_attn_args *p, void 
         return rc;
     if (!std::isfinite(p->scale)) return set_error(TMG_E_INVALID, "the scale must be finite");
     if (p->rows == 0 || kv->n_seq == 0) return TMG_OK;
-    const size_t need = kv4_attn_part_floats(view(kv), (int)p->rows, (int)p->nq) * 4;
+    const size_t need = kv4_attn_ws_bytes(view(kv), (int)p->rows, (int)p->nq);
     if (need && (!p->ws || p->ws_bytes < need || !aligned16(p->ws)))
         return set_error(TMG_E_INVALID, "the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
     StreamDevice dev;
     if ((rc = dev.enter((hipStream_t)stream, kv->data))) return rc;
-    if (p->k_new) {
-        const Kv4WriteArgs w{view(kv), p->k_new, p->v_new, new_stride, (int)p->rows, p->pos_dev, (int)p->pos};
-        if ((rc = launched(launch_kv4_write(w, (hipStream_t)stream), "tmg_kv4_attn"))) return rc;
-    }
     Kv4AttnArgs a{};
     a.c = view(kv);
     a.q = p->q;
@@ -184,6 +180,9 @@ extern "C" int tmg_kv4_attn(const tmg_kv4 *kv, const tmg_kv4_attn_args *p, void 
     a.rows = (int)p->rows;
     a.pos_dev = p->pos_dev;
     a.pos = (int)p->pos;
+    a.k_new = p->k_new;
+    a.v_new = p->v_new;
+    a.new_stride = new_stride;
     a.scale = p->scale != 0.0f ? p->scale : 1.0f / sqrtf((float)kv->hd);
-    return launched(launch_kv4_attn(a, (float *)p->ws, (hipStream_t)stream), "tmg_kv4_attn");
+    return launched(launch_kv4_attn(a, p->ws, (hipStream_t)stream), "tmg_kv4_attn");
 }

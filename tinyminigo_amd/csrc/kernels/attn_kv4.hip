@@ -29,6 +29,7 @@
 // sequence is row c / group, head c % group.
 #include <algorithm>
 
+#include "coh.cuh"
 #include "kv4.cuh"
 
 namespace tmg {
@@ -47,31 +48,45 @@ constexpr int kQParts = 6;
 template <int HD>
 struct Kv4Query {
     static constexpr int KH = (HD + 127) / 128;
+    f32x16 ev[KH], od[KH];  // the lane's even and odd dimensions, until split
     u32x6 part[KH][kQParts];
     uint32_t scale[KH][2];  // part n's byte: byte n & 3 of word n >> 2
 
-    // src: the column's HD floats, or null for a column that does not exist
-    __device__ __forceinline__ void load(const float *src, int lg, float mul) {
+    // src: the column's HD floats.  Lanes past the head's dimensions repeat
+    // the first ones; split() takes them as zeros.  (No branch: a loaded value
+    // that meets a constant is waited for on the spot.)
+    __device__ __forceinline__ void fetch(const float *src, int lg) {
 #pragma unroll
         for (int h = 0; h < KH; h++) {
-            f32x16 ev, od;
+            const float *p = src + (128 * h + 32 * lg < HD ? 128 * h + 32 * lg : 0);
 #pragma unroll
-            for (int i = 0; i < 16; i++) ev[i] = od[i] = 0.f;
-            const int d0 = 128 * h + 32 * lg;
-            if (src && d0 < HD) {
-#pragma unroll
-                for (int i = 0; i < (HD < 32 ? HD : 32) / 4; i++) {
-                    const f32x4 v = *reinterpret_cast<const f32x4 *>(src + d0 + 4 * i);
-                    ev[2 * i] = v.x * mul;
-                    od[2 * i] = v.y * mul;
-                    ev[2 * i + 1] = v.z * mul;
-                    od[2 * i + 1] = v.w * mul;
+            for (int i = 0; i < 8; i++) {
+                if (4 * i < HD) {
+                    const f32x4 v = *reinterpret_cast<const f32x4 *>(p + 4 * i);
+                    ev[h][2 * i] = v.x;
+                    od[h][2 * i] = v.y;
+                    ev[h][2 * i + 1] = v.z;
+                    od[h][2 * i + 1] = v.w;
+                } else {
+                    ev[h][2 * i] = ev[h][2 * i + 1] = od[h][2 * i] = od[h][2 * i + 1] = 0.f;
                 }
             }
+        }
+    }
+
+    // Scales by f and splits.
+    __device__ __forceinline__ void split(float f, int lg) {
+#pragma unroll
+        for (int h = 0; h < KH; h++) {
+            // (a NaN or an infinity times the zero marks a column that is NaN anyway)
+            const float mul = 128 * h + 32 * lg < HD ? f : 0.f;
             uint32_t m = 0;
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                m = max(m, max(__float_as_uint(ev[i]) & 0x7FFFFFFFu, __float_as_uint(od[i]) & 0x7FFFFFFFu));
+            for (int i = 0; i < 16; i++) {
+                ev[h][i] *= mul;
+                od[h][i] *= mul;
+                m = max(m, max(__float_as_uint(ev[h][i]) & 0x7FFFFFFFu, __float_as_uint(od[h][i]) & 0x7FFFFFFFu));
+            }
             // the largest magnitude within (3.75, 7.5] of the first part's scale
             int e = (int)(m >> 23) - 2 + ((m & 0x7FFFFFu) > 0x700000u);
             e = min(max(e, 27), 252);
@@ -81,13 +96,13 @@ struct Kv4Query {
 #pragma unroll
             for (int n = 0; n < kQParts; n++) {
                 const float s = __uint_as_float((uint32_t)(e - 4 * n) << 23);
-                part[h][n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(ev, od, s);
+                part[h][n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(ev[h], od[h], s);
                 if (n + 1 < kQParts) {
                     const f32x32 v = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(part[h][n], s);
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        ev[i] -= v[2 * i];
-                        od[i] -= v[2 * i + 1];
+                        ev[h][i] -= v[2 * i];
+                        od[h][i] -= v[2 * i + 1];
                     }
                 }
             }
@@ -101,22 +116,19 @@ struct Kv4Key {
     u32x4 code[KH];
     uint32_t scale[KH];
 
-    __device__ __forceinline__ void load(const Kv4Planes<HD> &pl, size_t row, int lg) {
+    // Codes and scales at the row `row` of their planes.  Lanes past the
+    // head's dimensions repeat the first ones, against zeros of the query.
+    __device__ __forceinline__ void load(const uint8_t *kc, const uint8_t *ks, unsigned row, int lg) {
 #pragma unroll
         for (int h = 0; h < KH; h++) {
-            code[h] = u32x4{0, 0, 0, 0};
-            scale[h] = 127;
-            if (128 * h + 32 * lg < HD) {
-                const uint8_t *p = pl.kc + row * (HD / 2) + 64 * h + 16 * lg;
-                if constexpr (HD == 16) {
-                    const uint2 c = *reinterpret_cast<const uint2 *>(p);
-                    code[h].x = c.x;
-                    code[h].y = c.y;
-                } else {
-                    code[h] = *reinterpret_cast<const u32x4 *>(p);
-                }
-                scale[h] = pl.ks[row * kv4_groups(HD) + 4 * h + lg];
+            const unsigned at = 128 * h + 32 * lg < HD ? 4 * h + lg : 0;
+            if constexpr (HD == 16) {
+                const uint2 c = *reinterpret_cast<const uint2 *>(kc + row * (HD / 2));
+                code[h] = u32x4{c.x, c.y, 0, 0};
+            } else {
+                code[h] = *reinterpret_cast<const u32x4 *>(kc + (row * (HD / 2) + 16 * at));
             }
+            scale[h] = ks[row * kv4_groups(HD) + at];
         }
     }
 };
@@ -154,12 +166,12 @@ struct Kv4Values {
     uint32_t code[8][W];
     uint32_t scale[8];
 
-    // row0: the head's first row; keys past `last` repeat it
-    __device__ __forceinline__ void load(const Kv4Planes<HD> &pl, size_t row0, int key0, int last, int r, int lg) {
+    // Row d and those after it repeat row d of the planes' first 32.
+    __device__ __forceinline__ void load(const uint8_t *vc, const uint8_t *vs, int d, int r, int lg) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const size_t row = row0 + min(key0 + 16 * (j >> 2) + 4 * lg + (j & 3), last);
-            const uint8_t *p = pl.vc + row * (HD / 2);
+            const unsigned row = (unsigned)min(16 * (j >> 2) + 4 * lg + (j & 3), d);
+            const uint8_t *p = vc + row * (HD / 2);
             if constexpr (HD == 256) {
                 const uint2 c = *reinterpret_cast<const uint2 *>(p + 8 * r);
                 code[j][0] = c.x;
@@ -171,9 +183,9 @@ struct Kv4Values {
             } else if constexpr (HD == 32) {
                 code[j][0] = p[r];
             } else {
-                code[j][0] = (uint32_t)p[r >> 1] >> (4 * (r & 1));
+                code[j][0] = p[r >> 1];
             }
-            scale[j] = pl.vs[row * kv4_groups(HD) + r * DPL / 32];
+            scale[j] = vs[row * kv4_groups(HD) + r * DPL / 32];
         }
     }
 
@@ -202,9 +214,11 @@ struct Kv4Values {
         for (int j = 0; j < 8; j++)
             w[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(
                                                     code[j][I / 4], kv4_scale(scale[j]), I & 3));
+        // a lane's one dimension of 16 is half of the byte it read
+        const uint32_t pick = HD == 16 && (threadIdx.x & 1) ? 0x07060302u : 0x05040100u;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            even[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x05040100u);
+            even[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], pick);
             odd[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
         }
     }
@@ -248,18 +262,18 @@ __device__ __forceinline__ void kv4_values(const Kv4Values<HD> &v, const bf16x8 
 
 // NaN into the outputs of the columns that see a marked group's key: lane
 // (r, lg) holds dimensions (4 lg + i) HD / 16 + t of column r, which are those
-// of the lanes (4 lg + i, any) of `bits`.
-template <int HD>
-__device__ __forceinline__ void nan_values(uint32_t bits, int key0, int qpos, int lg, f32x4 (&o)[HD / 16]) {
+// of the lanes (4 lg + i, any) of marked(j), the lanes whose key j is marked.
+template <int HD, class F>
+__device__ __forceinline__ void nan_values(F marked, int key0, int qpos, int lg, f32x4 (&o)[HD / 16]) {
 #pragma unroll 1
     for (int j = 0; j < 8; j++) {
-        const unsigned long long marked = __builtin_amdgcn_ballot_w64((bits >> j) & 1);
+        const unsigned long long lanes = marked(j);
 #pragma unroll 1
         for (int kl = 0; kl < 4; kl++) {
             if (key0 + 16 * (j >> 2) + 4 * kl + (j & 3) > qpos) continue;
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                if ((marked >> (16 * kl + 4 * lg + i)) & 1)
+                if ((lanes >> (16 * kl + 4 * lg + i)) & 1)
 #pragma unroll
                     for (int t = 0; t < HD / 16; t++) o[t][i] = __builtin_nanf("");
         }
@@ -307,185 +321,482 @@ __device__ __forceinline__ void kv4_store(const Kv4AttnArgs &a, int seq, int row
     if (a.out_hi) split_bf16(v, a.out_hi + i, a.out_lo + i);
 }
 
-// The blocks [b0, b1) of nb that split `sp` takes of `active`.
-__device__ __forceinline__ int split_begin(int nb, int sp, int active) { return (int)((int64_t)nb * sp / active); }
+// A new row of one head, quantized by a wavefront, in LDS in the cache's layout.
+template <int HD>
+struct Kv4NewRow {
+    static constexpr int NG = kv4_groups(HD), LPR = HD / 8, W = Kv4Values<HD>::W;
+    union {
+        uint32_t code[2][LPR];
+        u32x4 key16[2 * LPR / 4 ? 2 * LPR / 4 : 1];
+    };
+    uint8_t scale[2][8];
 
-// Few columns: a workgroup owns a tile of 16 columns and a run of blocks of
-// 128 keys, of which each wavefront takes a unit of 32, with a softmax state
-// of its own; the wavefronts are merged through LDS, the runs (splits) by
-// kv4_combine_kernel.
+    // Lanes [0, LPR) take the key, the next LPR the value; x: the lane's
+    // eight floats.  Also written to the cache's row.
+    __device__ __forceinline__ void put(const float (&x)[8], int lane, const Kv4Planes<HD> &pl, size_t row) {
+        const int i = lane / LPR, at = lane % LPR;
+        uint32_t byte;
+        const uint32_t c = kv4_quantize8<LPR / NG>(x, &byte);
+        if (i < 2) {
+            code[i][at] = c;
+            *reinterpret_cast<uint32_t *>((i ? pl.vc : pl.kc) + row * (HD / 2) + at * 4) = c;
+            if (at % (LPR / NG) == 0) {
+                scale[i][at / (LPR / NG)] = (uint8_t)byte;
+                (i ? pl.vs : pl.ks)[row * NG + at / (LPR / NG)] = (uint8_t)byte;
+            }
+        }
+    }
+    // The row in the place of row `at` of a unit that was loaded.
+    __device__ __forceinline__ void patch(Kv4Key<HD> (&k)[2], Kv4Values<HD> &v, int at, int r, int lg) const {
+        if (r == (at & 15)) {
+#pragma unroll
+            for (int h = 0; h < Kv4Key<HD>::KH; h++) {
+                const int w = 128 * h + 32 * lg < HD ? 4 * h + lg : 0;
+                const u32x4 c = HD == 16 ? u32x4{code[0][0], code[0][1], 0, 0} : key16[w];
+                const uint32_t sc = scale[0][w];
+                if (at < 16) {
+                    k[0].code[h] = c;
+                    k[0].scale[h] = sc;
+                } else {
+                    k[1].code[h] = c;
+                    k[1].scale[h] = sc;
+                }
+            }
+        }
+        const uint8_t *p = reinterpret_cast<const uint8_t *>(code[1]);
+        uint32_t c[W];
+        if constexpr (HD == 256) {
+            c[0] = code[1][2 * r];
+            c[1] = code[1][2 * r + 1];
+        } else if constexpr (HD == 128) {
+            c[0] = code[1][r];
+        } else if constexpr (HD == 64) {
+            c[0] = reinterpret_cast<const uint16_t *>(p)[r];
+        } else {
+            c[0] = p[HD == 32 ? r : r >> 1];
+        }
+        const uint32_t sc = scale[1][r * Kv4Values<HD>::DPL / 32];
+        const bool mine = lg == ((at >> 2) & 3);
+        const int slot = (at >> 4) * 4 + (at & 3);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const bool here = mine && j == slot;
+#pragma unroll
+            for (int w = 0; w < W; w++) v.code[j][w] = here ? c[w] : v.code[j][w];
+            v.scale[j] = here ? sc : v.scale[j];
+        }
+    }
+};
+
+// x / group for x below 2^21, by the reciprocal the host gives.
+__device__ __forceinline__ int div_group(const Kv4AttnArgs &a, int x) { return (int)(((float)x + 0.5f) * a.inv_group); }
+
+// An item is a tile of 16 columns of one sequence: the sequence's columns
+// 16 tile .. + cols - 1, the first of them head h0 of query row t0.
+struct Kv4Item {
+    int seq, tile, cols, t0, h0;
+    int pos;   // the sequence's first row position, or -1
+    int last;  // the tile's last position
+    int nb;    // blocks of keys up to it
+};
+
+template <int BLOCK>
+__device__ __forceinline__ Kv4Item kv4_item(const Kv4AttnArgs &a, int i) {
+    Kv4Item it;
+    it.seq = a.ntile == 1 ? i : i / a.ntile;
+    it.tile = i - it.seq * a.ntile;
+    it.cols = min(16, a.rows * a.group - 16 * it.tile);
+    it.t0 = a.ntile == 1 ? 0 : 16 * it.tile / a.group;
+    it.h0 = 16 * it.tile - it.t0 * a.group;
+    it.pos = kv4_pos(a.pos_dev, a.pos, it.seq, a.rows, a.c.cap);
+    it.last = it.pos + it.t0 + div_group(a, it.h0 + it.cols - 1);
+    it.nb = it.pos < 0 ? 0 : it.last / BLOCK + 1;
+    return it;
+}
+
+// Output element d of the item's column c.
+template <int HD>
+__device__ __forceinline__ void kv4_put(const Kv4AttnArgs &a, const Kv4Item &it, int g, int c, int d, float O, float L) {
+    const int dt = div_group(a, it.h0 + c), h = it.h0 + c - dt * a.group;
+    const size_t i = ((size_t)it.seq * a.rows + it.t0 + dt) * a.out_stride + (size_t)(g * a.group + h) * HD + d;
+    const float v = L == 0.f ? 0.f : O / L;
+    if (a.out) a.out[i] = v;
+    if (a.out_hi) split_bf16(v, a.out_hi + i, a.out_lo + i);
+}
+
+// Wavefronts of a workgroup; a wavefront takes 32 keys of a block.
+template <int HD>
+constexpr int kv4_waves() {
+    return HD == 256 ? 4 : 8;  // at 256 its registers leave room for one a SIMD
+}
+
+// A workgroup owns one KV head and a run of blocks (32 keys a wavefront), each
+// wavefront with a softmax state of its own; the wavefronts are merged through
+// LDS.  Where an item's blocks are dealt to several workgroups, the last of
+// them to arrive merges their states, in the order of the runs, so that the
+// result does not depend on who is last: one launch in all.
+//
+// - ONE item: the workgroups take the blocks in turn.  A workgroup's first
+//   block does not hang on the position, so its keys are loaded before the
+//   position, which may live on the device, is known.
+// - Up to kKv4FlatItems items (a.flat): the items' blocks, one after the other, are cut
+//   into equal runs, whatever the sequences' lengths are; a run ends in the
+//   middle of an item and goes on with the next.  (The same number of
+//   workgroups for every item left sequences of 65 to 131070 positions at 100
+//   us, 1.9 times the time of their mean.)
+// - More items: a workgroup each.
+//
+// With a.k_new (one row a sequence) the wavefront that owns the new position
+// quantizes the row, stores it and takes it from LDS; no other needs it.
 //
 // Bound by the latency of its loads and of the merge for one sequence, by the
 // cache's bytes for many.
-template <int HD>
-__global__ __launch_bounds__(kBlock, 2) void kv4_attn_rows_kernel(const Kv4AttnArgs a) {
-    constexpr int DPL = HD / 16, PAD = 4;
-    __shared__ __attribute__((aligned(16))) float s_o[4][16][HD + PAD];
-    __shared__ float s_m[4][16], s_l[4][16];
-    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, r = lane & 15, lg = lane >> 4;
-    const int group = a.nq / a.c.nkv, ncol = a.rows * group, ntile = (ncol + 15) / 16;
-    const int g = (int)(blockIdx.x % (unsigned)a.c.nkv);
-    unsigned rest = blockIdx.x / (unsigned)a.c.nkv;
-    const int sp = (int)(rest % (unsigned)a.nsplit);
-    rest /= (unsigned)a.nsplit;
-    const int tile = (int)(rest % (unsigned)ntile), seq = (int)(rest / (unsigned)ntile);
-    const int cols = min(16, ncol - 16 * tile);
-    const int pos = kv4_pos(a.pos_dev, a.pos, seq, a.rows, a.c.cap);
-    const int row_r = (16 * tile + min(r, cols - 1)) / group, head_r = (16 * tile + min(r, cols - 1)) % group;
-    const int last = pos + (16 * tile + cols - 1) / group;  // the tile's last position
-    const int nb = pos < 0 ? 0 : last / kKv4Block + 1;
-    const int active = min(a.nsplit, nb);
-    if (sp >= max(active, 1) || (pos < 0 && a.nsplit > 1)) return;  // idle rows of split launches: the merge's
+template <int HD, bool ONE>
+__global__ __launch_bounds__(64 * kv4_waves<HD>()) void kv4_attn_rows_kernel(const Kv4AttnArgs a) {
+    constexpr int DPL = HD / 16, PITCH = HD + 4, NW = kv4_waves<HD>(), NT = 64 * NW, BLOCK = 32 * NW;
+    // the wavefronts' sums [NW][16][PITCH], then the runs' weights [16][kKv4MaxRuns]
+    constexpr int SUMS = NW * 16 * PITCH, WEIGHTS = 16 * kKv4MaxRuns;
+    __shared__ __attribute__((aligned(16))) float s_o[SUMS > WEIGHTS ? SUMS : WEIGHTS];
+    __shared__ float s_m[16][NW], s_l[16][NW];
+    __shared__ Kv4NewRow<HD> s_new;
+    __shared__ unsigned s_arrived;
+    __shared__ int s_first[ONE ? 1 : kKv4FlatItems + 1];  // the items' first blocks in the row of all
+    __shared__ int s_sum[NW], s_start;
+    __shared__ float s_red[NT];
+    const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r = lane & 15, lg = lane >> 4;
+    const int g = (int)(blockIdx.x % (unsigned)a.c.nkv), run = (int)(blockIdx.x / (unsigned)a.c.nkv);
+    const size_t row0 = (size_t)g * a.c.cap;
+    const bool append = a.k_new != nullptr;
 
-    Kv4State<HD> st;
-    if (pos >= 0) {
-        const Kv4Planes<HD> pl(a.c, seq);
-        const size_t row0 = (size_t)g * a.c.cap;
-        const int qpos = r < cols ? pos + row_r : -1;
-        const int first_pos = pos + 16 * tile / group;
-        const int b1 = split_begin(nb, sp + 1, active);
-        Kv4Key<HD> k[2];
-        Kv4Values<HD> v;
-        auto load = [&](int key0) {
-            k[0].load(pl, row0 + min(key0 + r, last), lg);
-            k[1].load(pl, row0 + min(key0 + 16 + r, last), lg);
-            v.load(pl, row0, key0, last, r, lg);
-        };
-        int key0 = split_begin(nb, sp, active) * kKv4Block + 32 * wave;
-        const int end = min(b1 * kKv4Block, last + 1);
-        if (key0 < end) load(key0);
-        Kv4Query<HD> q;
-        q.load(r < cols ? a.q + ((size_t)seq * a.rows + row_r) * a.q_stride + (size_t)(g * group + head_r) * HD : nullptr,
-               lg, a.scale * 1.4426950408889634f);
-        for (; key0 < end; key0 += kKv4Block) {
-            f32x4 s[2] = {kv4_scores(k[0], q), kv4_scores(k[1], q)};
-            Kv4Values<HD> vn = v;
-            if (key0 + kKv4Block < end) load(key0 + kKv4Block);
-            if (key0 + 31 > first_pos || cols < 16) {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (key0 + 16 * (j >> 2) + 4 * lg + (j & 3) > qpos) s[j >> 2][j & 3] = -INFINITY;
-            }
-            float p[8];
-            st.weights(s, p);
-            bf16x8 pp[3];
-            split_p(p, pp);
-            uint32_t bad;
-            const bool any_bad = vn.take_bad(&bad);
-            kv4_values(vn, pp, st.o);
-            if (any_bad) nan_values<HD>(bad, key0, qpos, lg, st.o);
+    Kv4Key<HD> k[2];
+    Kv4Values<HD> v;
+    Kv4Query<HD> q;
+    float xn[8];
+    // keys key0 .. +31 of the head; those past lim repeat it
+    auto load = [&](const Kv4Planes<HD> &pl, int key0, int lim) {
+        const int at = min(key0, lim), d = lim - at;
+        const size_t row = row0 + at;
+        const uint8_t *const kc = pl.kc + row * (HD / 2), *const ks = pl.ks + row * kv4_groups(HD);
+        k[0].load(kc, ks, (unsigned)min(r, d), lg);
+        k[1].load(kc, ks, (unsigned)min(16 + r, d), lg);
+        v.load(pl.vc + row * (HD / 2), pl.vs + row * kv4_groups(HD), d, r, lg);
+    };
+    auto fetch = [&](int seq, int t0, int h0, int cols) {
+        const int c = h0 + min(r, cols - 1), dt = div_group(a, c), h = c - dt * a.group;
+        q.fetch(a.q + ((size_t)seq * a.rows + t0 + dt) * a.q_stride + (size_t)(g * a.group + h) * HD, lg);
+        if (append) {
+            const int l = lane % (HD / 4);
+            const float *src = (l < HD / 8 ? a.k_new : a.v_new) + (size_t)seq * a.new_stride + (size_t)g * HD + l % (HD / 8) * 8;
+            *reinterpret_cast<f32x4 *>(xn) = *reinterpret_cast<const f32x4 *>(src);
+            *reinterpret_cast<f32x4 *>(xn + 4) = *reinterpret_cast<const f32x4 *>(src + 4);
         }
-    }
-    // the wavefronts' states
-    st.l = add_xor32(add_xor16(st.l));
-    if (r < cols) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int d = 0; d < DPL; d++) s_o[wave][r][(4 * lg + i) * DPL + d] = st.o[d][i];
-        if (lg == 0) {
-            s_m[wave][r] = st.m;
-            s_l[wave][r] = st.l;
-        }
-    }
-    __syncthreads();
-    const size_t pbase = ((((size_t)seq * ntile + tile) * a.c.nkv + g) * a.nsplit + sp) * a.part_cols;
-    for (int idx = t; idx < cols * HD; idx += kBlock) {
-        const int c = idx / HD, d = idx % HD;
-        float M = s_m[0][c];
-#pragma unroll
-        for (int w = 1; w < 4; w++) M = fmaxf(M, s_m[w][c]);
-        float L = 0.f, O = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            // a wavefront without a finite maximum still brings its sums: they
-            // are zeros, or NaN
-            const float f = s_m[w][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[w][c] - M);
-            L = fmaf(s_l[w][c], f, L);
-            O = fmaf(s_o[w][c][d], f, O);
-        }
-        if (active <= 1) {
-            const int row = (16 * tile + c) / group, h = (16 * tile + c) % group;
-            kv4_store(a, seq, row, (g * group + h) * HD + d, L == 0.f ? 0.f : O / L);
-        } else {
-            a.part[(pbase + c) * HD + d] = O;
-            if (d == 0) {
-                a.part_ml[(pbase + c) * 2] = M;
-                a.part_ml[(pbase + c) * 2 + 1] = L;
-            }
-        }
-    }
-}
+    };
 
-// Merge of the splits of a tile of columns: workgroup (column, (sequence,
-// tile, KV head)).
-__global__ __launch_bounds__(kBlock) void kv4_combine_kernel(const Kv4AttnArgs a) {
-    const int group = a.nq / a.c.nkv, ncol = a.rows * group, ntile = (ncol + a.tile_cols - 1) / a.tile_cols;
-    const int g = (int)(blockIdx.x % (unsigned)a.c.nkv);
-    unsigned rest = blockIdx.x / (unsigned)a.c.nkv;
-    const int tile = (int)(rest % (unsigned)ntile), seq = (int)(rest / (unsigned)ntile);
-    const int cols = min(a.tile_cols, ncol - a.tile_cols * tile);
-    const int c = blockIdx.y;
-    if (c >= cols) return;
-    const int pos = kv4_pos(a.pos_dev, a.pos, seq, a.rows, a.c.cap);
-    const int nb = pos < 0 ? 0 : (pos + (a.tile_cols * tile + cols - 1) / group) / kKv4Block + 1;
-    const int active = min(a.nsplit, nb);
-    if (active == 1) return;  // written by the split itself
-    const int row = (a.tile_cols * tile + c) / group, h = (a.tile_cols * tile + c) % group;
-    const size_t base = (((size_t)seq * ntile + tile) * a.c.nkv + g) * a.nsplit * a.part_cols + c;
-    for (int d = threadIdx.x; d < a.c.hd; d += kBlock) {
-        float M = -INFINITY, L = 0.f, O = 0.f;
-        for (int s = 0; s < active; s++) M = fmaxf(M, a.part_ml[(base + (size_t)s * a.part_cols) * 2]);
-        for (int s = 0; s < active; s++) {
-            const size_t p = base + (size_t)s * a.part_cols;
-            const float m = a.part_ml[p * 2], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-            L = fmaf(a.part_ml[p * 2 + 1], f, L);
-            O = fmaf(a.part[p * a.c.hd + d], f, O);
+    int item = 0, x = 0, xend = 1;  // blocks [x, xend) of all the items'
+    int per = 1, total = 0;         // blocks of a run, of all items
+    const bool flat = !ONE && a.flat;
+    if constexpr (ONE) {
+        // the query first: it is split while the first keys are on their way
+        fetch(0, 0, 0, min(16, a.rows * a.group));
+        load(Kv4Planes<HD>(a.c, 0), run * BLOCK + 32 * wave, (int)a.c.cap - 1);
+        asm volatile("" ::: "memory");  // not behind the position's read
+    } else if (flat) {
+        constexpr int PER = (kKv4FlatItems + NT - 1) / NT;
+        int n[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            n[i] = t * PER + i < a.items ? max(1, kv4_item<BLOCK>(a, t * PER + i).nb) : 0;
+            sum += n[i];
         }
-        kv4_store(a, seq, row, (g * group + h) * a.c.hd + d, L == 0.f ? 0.f : O / L);
+        int before = sum;  // over the wavefront's lanes up to this one
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int o = __shfl_up(before, off, 64);
+            before += lane >= off ? o : 0;
+        }
+        if (lane == 63) s_sum[wave] = before;
+        before -= sum;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const int o = s_sum[w];
+            before += w < wave ? o : 0;
+            total += o;
+        }
+        total = __builtin_amdgcn_readfirstlane(total);
+        per = (int)(((unsigned)total + (unsigned)a.runs - 1) / (unsigned)a.runs);
+        if ((int64_t)run * per >= total) return;
+        x = run * per;
+        xend = min(x + per, total);
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            if (t * PER + i <= a.items) s_first[t * PER + i] = before;
+            if (x >= before && x < before + n[i]) s_start = t * PER + i;
+            before += n[i];
+        }
+        if (t == 0) s_first[a.items] = total;
+        __syncthreads();
+        item = __builtin_amdgcn_readfirstlane(s_start);
+    } else {
+        item = run;
+    }
+    const int x_begin = x;
+    for (; x < xend; item++) {
+        const Kv4Item it = kv4_item<BLOCK>(a, item);
+        const Kv4Planes<HD> pl(a.c, it.seq);
+        // this workgroup's blocks b, b + step, .. < bend of the item, which
+        // `parts` workgroups share, the first of them run r0
+        int b = 0, bend = it.nb, step = 1, parts = 1, r0 = run;
+        bool begun = false;  // the run begins the item after another
+        if constexpr (ONE) {
+            if (it.nb > kKv4WholeBlocks) {
+                const unsigned each = ((unsigned)it.nb + a.runs - 1) / (unsigned)a.runs;
+                parts = (int)(((unsigned)it.nb + each - 1) / each);
+            }
+            if (run >= parts) return;
+            b = run;
+            step = parts;
+            r0 = 0;
+        } else if (flat) {
+            const int first = __builtin_amdgcn_readfirstlane(s_first[item]);
+            const int next = __builtin_amdgcn_readfirstlane(s_first[item + 1]);
+            b = x - first;
+            bend = min(min(xend, next) - first, it.nb);
+            if (x > first || xend < next) {
+                r0 = (int)((unsigned)first / (unsigned)per);
+                parts = (int)((unsigned)(next - 1) / (unsigned)per) - r0 + 1;
+                begun = x_begin < first;
+            }
+            x = min(xend, next);
+        }
+        if (!flat) xend = 0;
+        const int cols = it.cols, pos = it.pos;
+        Kv4State<HD> st;
+        if (pos >= 0) {
+            const int qpos = r < cols ? pos + it.t0 + div_group(a, it.h0 + r) : -1;
+            const int first_pos = pos + it.t0;
+            int key0 = b * BLOCK + 32 * wave;
+            const int end = min(bend * BLOCK, it.last + 1);
+            if constexpr (!ONE) {
+                fetch(it.seq, it.t0, it.h0, cols);
+                load(pl, key0, it.last);
+            }
+            q.split(a.scale * 1.4426950408889634f, lg);
+            for (; key0 < end; key0 += step * BLOCK) {
+                if (append && key0 + 31 >= pos) {
+                    s_new.put(xn, lane, pl, row0 + pos);
+                    // the wavefront's own LDS writes, in order
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                    s_new.patch(k, v, pos - key0, r, lg);
+                }
+                f32x4 s[2] = {kv4_scores(k[0], q), kv4_scores(k[1], q)};
+                Kv4Values<HD> vn = v;
+                if (key0 + step * BLOCK < end) load(pl, key0 + step * BLOCK, it.last);
+                if (key0 + 31 > first_pos || cols < 16) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (key0 + 16 * (j >> 2) + 4 * lg + (j & 3) > qpos) s[j >> 2][j & 3] = -INFINITY;
+                }
+                float p[8];
+                st.weights(s, p);
+                bf16x8 pp[3];
+                split_p(p, pp);
+                uint32_t bad;
+                const bool any_bad = vn.take_bad(&bad);
+                kv4_values(vn, pp, st.o);
+                if (any_bad)
+                    nan_values<HD>([&](int j) { return __builtin_amdgcn_ballot_w64((bad >> j) & 1); }, key0, qpos, lg, st.o);
+            }
+        }
+        // the wavefronts' states
+        st.l = add_xor32(add_xor16(st.l));
+        if (r < cols) {
+            float *const dst = s_o + (wave * 16 + r) * PITCH + 4 * lg * DPL;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int d = 0; d < DPL; d++) dst[i * DPL + d] = st.o[d][i];
+            if (lg == 0) {
+                s_m[r][wave] = st.m;
+                s_l[r][wave] = st.l;
+            }
+        }
+        __syncthreads();
+        // partial states: two slots a run, the second for an item that the
+        // run begins after another
+        const size_t slot = ((size_t)g * a.runs + run) * 2 + (begun ? 1 : 0);
+        for (int idx = t; idx < cols * HD; idx += NT) {
+            const int c = idx / HD, d = idx % HD;
+            float M = s_m[c][0];
+#pragma unroll
+            for (int w = 1; w < NW; w++) M = fmaxf(M, s_m[c][w]);
+            float L = 0.f, O = 0.f;
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                // a wavefront without a finite maximum still brings its sums:
+                // they are zeros, or NaN
+                const float f = s_m[c][w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[c][w] - M);
+                L = fmaf(s_l[c][w], f, L);
+                O = fmaf(s_o[(w * 16 + c) * PITCH + d], f, O);
+            }
+            if (parts == 1) {
+                kv4_put<HD>(a, it, g, c, d, O, L);
+            } else {
+                st_dev(a.part + (slot * a.part_cols + c) * HD + d, O);
+                if (d == 0) {
+                    st_dev(a.part_ml + (slot * a.part_cols + c) * 2, M);
+                    st_dev(a.part_ml + (slot * a.part_cols + c) * 2 + 1, L);
+                }
+            }
+        }
+        if (parts > 1) {
+            // a workgroup's partial state is complete before it counts itself
+            // in; no other shared item starts in r0
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            unsigned *const count = a.arrived + (size_t)g * a.runs + r0;
+            if (t == 0) s_arrived = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (s_arrived == (unsigned)parts - 1) {
+                if (t == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                // part i is run r0 + i, in its first slot but for a run that
+                // came to the item after another, which only r0 can
+                const bool late0 = flat && r0 * per < s_first[item];
+                const size_t slot0 = ((size_t)g * a.runs + r0) * 2;
+                auto part = [&](int i) { return (slot0 + 2 * (size_t)i + (i == 0 && late0 ? 1 : 0)) * a.part_cols; };
+                // SUB threads an element, each with the parts sub, sub + SUB,
+                // ..; its first parts are on their way while the columns'
+                // weights and sums are made
+                constexpr int FAR = kKv4MaxRuns / 64, AHEAD = 16;
+                const int elems = cols * HD, SUB = max(1, NT / elems);
+                const int e0 = SUB == 1 ? t : t % elems, sub = SUB == 1 ? 0 : t / elems;
+                float ahead[AHEAD];
+                auto grab = [&](int e, int i) {
+                    const float *src = a.part + (size_t)(e / HD) * HD + e % HD;
+#pragma unroll
+                    for (int u = 0; u < AHEAD; u++) ahead[u] = ld_dev(src + part(min(i + u * SUB, parts - 1)) * HD);
+                };
+                const bool busy = sub < SUB && e0 < elems;
+                if (busy) grab(e0, sub);
+                for (int c = wave; c < cols; c += NW) {
+                    float M = -INFINITY, L = 0.f, m[FAR], l[FAR];
+#pragma unroll
+                    for (int i = 0; i < FAR; i++) {
+                        const float *ml = a.part_ml + (part(min(lane + 64 * i, parts - 1)) + c) * 2;
+                        m[i] = ld_dev(ml);
+                        l[i] = ld_dev(ml + 1);
+                    }
+#pragma unroll
+                    for (int i = 0; i < FAR; i++) M = fmaxf(M, m[i]);
+                    M = wave_max(M);
+#pragma unroll
+                    for (int i = 0; i < FAR; i++) {
+                        const bool there = lane + 64 * i < parts;
+                        const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - M);
+                        L = there ? fmaf(l[i], f, L) : L;
+                        if (there) s_o[c * kKv4MaxRuns + lane + 64 * i] = f;
+                    }
+                    L = wave_sum(L);
+                    if (lane == 0) s_l[c][0] = L;
+                }
+                __syncthreads();
+                bool fresh = true;
+                for (int e = e0; busy && e < elems; e += NT) {
+                    const int c = e / HD;
+                    float O = 0.f;
+                    for (int i = sub; i < parts; i += AHEAD * SUB) {
+                        if (!fresh) grab(e, i);
+                        fresh = false;
+#pragma unroll
+                        for (int u = 0; u < AHEAD; u++)
+                            if (i + u * SUB < parts) O = fmaf(ahead[u], s_o[c * kKv4MaxRuns + i + u * SUB], O);
+                    }
+                    if (SUB == 1)
+                        kv4_put<HD>(a, it, g, c, e % HD, O, s_l[c][0]);
+                    else
+                        s_red[sub * elems + e] = O;
+                }
+                if (SUB > 1) {
+                    __syncthreads();
+                    if (t < elems) {
+                        float O = s_red[t];
+                        for (int i = 1; i < SUB; i++) O += s_red[i * elems + t];
+                        kv4_put<HD>(a, it, g, t / HD, t % HD, O, s_l[t / HD][0]);
+                    }
+                }
+            }
+        }
+        __syncthreads();
     }
 }
 
 }  // namespace
 
-Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq, uint32_t ctx) {
+Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq) {
     Kv4Plan p{};
     const int64_t ncol = (int64_t)rows * (nq / c.nkv);
-    p.tile_cols = 16;
-    p.part_cols = (int)std::min<int64_t>(p.tile_cols, ncol);
-    p.tiles = (ncol + p.tile_cols - 1) / p.tile_cols * c.nkv * c.n_seq;
-    const int64_t nb = ((int64_t)ctx + kKv4Block - 1) / kKv4Block;
-    p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({nb, (kKv4Workgroups + p.tiles - 1) / p.tiles, kKv4MaxSplits}));
+    p.part_cols = (int)std::min<int64_t>(16, ncol);
+    p.items = (ncol + 15) / 16 * c.n_seq;
+    const int block = c.hd == 256 ? 32 * kv4_waves<256>() : 32 * kv4_waves<128>();
+    const int64_t nb = ((int64_t)c.cap + block - 1) / block;
+    p.flat = p.items > 1 && p.items <= kKv4FlatItems && p.items * nb <= 1 << 30;
+    if (p.items > 1 && !p.flat) {
+        p.runs = (int)std::min<int64_t>(p.items, 0x7fffffff);
+    } else {
+        p.runs = (int)std::min<int64_t>({kKv4MaxRuns, p.items * nb, std::max(1, kKv4Workgroups / c.nkv)});
+        p.split = nb > 1 && p.runs > 1;
+    }
     return p;
 }
 
-size_t kv4_attn_part_floats(const Kv4Cache &c, int rows, int nq) {
-    // the number of splits does not fall as the context grows
-    const Kv4Plan p = plan_kv4_attn(c, rows, nq, c.cap);
-    return p.nsplit == 1 ? 0 : (size_t)p.tiles * p.nsplit * p.part_cols * (c.hd + 2);
+size_t kv4_attn_ws_bytes(const Kv4Cache &c, int rows, int nq) {
+    const Kv4Plan p = plan_kv4_attn(c, rows, nq);
+    return p.split ? kKv4CounterBytes + (size_t)2 * c.nkv * p.runs * p.part_cols * (c.hd + 2) * 4 : 0;
 }
 
-hipError_t launch_kv4_attn(Kv4AttnArgs a, float *ws, hipStream_t s) {
-    const uint32_t ctx = a.pos_dev ? a.c.cap : (uint32_t)(a.pos + a.rows);
-    const Kv4Plan p = plan_kv4_attn(a.c, a.rows, a.nq, ctx);
-    if (p.tiles * p.nsplit > 0x7fffffff || (p.nsplit > 1 && !ws)) return hipErrorInvalidValue;
-    a.nsplit = p.nsplit;
-    a.tile_cols = p.tile_cols;
+namespace {
+
+template <int HD>
+void launch_rows(const Kv4AttnArgs &a, unsigned grid, hipStream_t s) {
+    const dim3 block(64 * kv4_waves<HD>());
+    if (a.items == 1)
+        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, true>), dim3(grid), block, 0, s, a);
+    else
+        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, false>), dim3(grid), block, 0, s, a);
+}
+
+}  // namespace
+
+hipError_t launch_kv4_attn(Kv4AttnArgs a, void *ws, hipStream_t s) {
+    const Kv4Plan p = plan_kv4_attn(a.c, a.rows, a.nq);
+    const int64_t grid = (int64_t)p.runs * a.c.nkv;
+    if (grid > 0x7fffffff || (p.split && !ws)) return hipErrorInvalidValue;
+    if (a.k_new && a.rows > 1) {
+        const Kv4WriteArgs w{a.c, a.k_new, a.v_new, a.new_stride, a.rows, a.pos_dev, a.pos};
+        const hipError_t e = launch_kv4_write(w, s);
+        if (e != hipSuccess) return e;
+        a.k_new = a.v_new = nullptr;
+    }
+    a.group = a.nq / a.c.nkv;
+    a.inv_group = 1.0f / (float)a.group;
+    a.ntile = (a.rows * a.group + 15) / 16;
+    a.items = (int)p.items;
+    a.flat = p.flat;
+    a.runs = p.runs;
     a.part_cols = p.part_cols;
-    a.part = ws;
-    a.part_ml = ws + (size_t)p.tiles * p.nsplit * p.part_cols * a.c.hd;
-    const dim3 grid((unsigned)(p.tiles * p.nsplit));
+    a.arrived = (unsigned *)ws;
+    a.part_ml = (float *)((char *)ws + kKv4CounterBytes);
+    a.part = a.part_ml + (size_t)2 * grid * p.part_cols * 2;
     switch (a.c.hd) {
-        case 16: hipLaunchKernelGGL((kv4_attn_rows_kernel<16>), grid, dim3(kBlock), 0, s, a); break;
-        case 32: hipLaunchKernelGGL((kv4_attn_rows_kernel<32>), grid, dim3(kBlock), 0, s, a); break;
-        case 64: hipLaunchKernelGGL((kv4_attn_rows_kernel<64>), grid, dim3(kBlock), 0, s, a); break;
-        case 128: hipLaunchKernelGGL((kv4_attn_rows_kernel<128>), grid, dim3(kBlock), 0, s, a); break;
-        case 256: hipLaunchKernelGGL((kv4_attn_rows_kernel<256>), grid, dim3(kBlock), 0, s, a); break;
+        case 16: launch_rows<16>(a, (unsigned)grid, s); break;
+        case 32: launch_rows<32>(a, (unsigned)grid, s); break;
+        case 64: launch_rows<64>(a, (unsigned)grid, s); break;
+        case 128: launch_rows<128>(a, (unsigned)grid, s); break;
+        case 256: launch_rows<256>(a, (unsigned)grid, s); break;
         default: return hipErrorInvalidValue;
     }
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.nsplit == 1) return e;
-    hipLaunchKernelGGL(kv4_combine_kernel, dim3((unsigned)p.tiles, p.part_cols), dim3(kBlock), 0, s, a);
     return hipGetLastError();
 }
+
 }  // namespace tmg

@@ -403,25 +403,37 @@ struct Kv4AttnArgs {
     const int *pos_dev;
     int pos;
     float scale;
-    // set by launch_kv4_attn: the column tiles' splits and their partial
-    // states [sequence][tile][KV head][split][part_cols] of hd floats in part
-    // and of (max, sum) in part_ml
-    int nsplit, tile_cols, part_cols;
+    // rows to append first ([nkv][hd], new_stride floats apart), or null
+    const float *k_new, *v_new;
+    size_t new_stride;
+    // set by launch_kv4_attn (see Kv4Plan): the runs' partial states [KV
+    // head][run][2][part_cols] of hd floats in part and of (max, sum) in
+    // part_ml, and per KV head and run the count of the arrived parts of the
+    // shared item that starts in it
+    int group, ntile, items, flat, runs, part_cols;
+    float inv_group;  // 1 / group
+    unsigned *arrived;
     float *part, *part_ml;
 };
-constexpr int kKv4Block = 128;       // positions per block of the splits
-constexpr int kKv4MaxSplits = 64;
-constexpr int kKv4Workgroups = 512;  // two per CU
+constexpr int kKv4Workgroups = 256;   // of 512 threads: one per CU
+constexpr int kKv4MaxRuns = 256;
+constexpr int kKv4FlatItems = 1024;   // more items than this are a workgroup each
+constexpr int kKv4WholeBlocks = 2;    // blocks that one workgroup takes rather than share
+// Counters of the shared items, one a workgroup at most, at the start of the
+// workspace.
+constexpr size_t kKv4CounterBytes = kKv4Workgroups * 4;
 struct Kv4Plan {
-    int tile_cols, part_cols;  // columns (query rows x heads of a KV head) of a workgroup, and of its partial states
-    int64_t tiles;             // column tiles of all sequences and KV heads
-    int nsplit;                // workgroups that share a tile's keys
+    int part_cols;  // columns (query rows x heads of a KV head) of an item's partial states
+    int64_t items;  // tiles of 16 columns of all sequences
+    int runs;       // workgroups of a KV head
+    bool flat;      // the items' blocks are cut into equal runs
+    bool split;     // an item may be shared by several workgroups
 };
-// The launch for contexts of up to ctx positions.
-Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq, uint32_t ctx);
-// Floats of the partial states, enough for every context of the cache.
-size_t kv4_attn_part_floats(const Kv4Cache &c, int rows, int nq);
-hipError_t launch_kv4_attn(Kv4AttnArgs a, float *ws, hipStream_t s);
+Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq);
+// Workspace enough for every position: counters, which are zero between
+// launches, then the partial states.
+size_t kv4_attn_ws_bytes(const Kv4Cache &c, int rows, int nq);
+hipError_t launch_kv4_attn(Kv4AttnArgs a, void *ws, hipStream_t s);
 
 // ---- sampling --------------------------------------------------------------
 

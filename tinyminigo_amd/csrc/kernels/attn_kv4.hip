@@ -6,11 +6,12 @@
 // Scores.  The cache's codes and scale bytes are what
 // v_mfma_scale_f32_16x16x128_f8f6f4 takes, so keys go from memory into the
 // matrix instruction as they are.  The query, scaled to log2 units, is the
-// sum of six 6-bit floats (e2m3) a dimension: part n holds what the parts
-// before it leave, at a sixteenth of the scale (each rounding leaves at most
-// a quarter of its part's step of 1/8 .. 1/2), so 2^-24 of the largest of 32
-// dimensions is left out, as f32 itself would.  A 4-bit and a 6-bit operand
-// run at four times the bf16 rate: six parts cost half of three bf16 ones.
+// sum of six 6-bit floats (e2m3) a dimension, of which the multiples of 1/8
+// up to 15/8 are used: digits of the fixed-point number that the largest of 32
+// dimensions scales to (-15 .. 15, then -8 .. 8 at each sixteenth of the
+// scale), so 2^-24 of the largest dimension is left out, as f32 itself would.
+// A 4-bit and a 6-bit operand run at four times the bf16 rate: six parts cost
+// half of three bf16 ones.
 //
 // Values.  A value's scale belongs to a (position, 32 dimensions), which the
 // instruction cannot take along its contracted axis, so values are widened to
@@ -44,6 +45,13 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kQParts = 6;
 
+// A barrier for LDS alone: loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // A column's query in a lane: 128-dimension halves, parts, scale bytes.
 template <int HD>
 struct Kv4Query {
@@ -74,8 +82,8 @@ struct Kv4Query {
         }
     }
 
-    // Scales by f and splits.
-    __device__ __forceinline__ void split(float f, int lg) {
+    // Scales by f, for digit().
+    __device__ __forceinline__ void ready(float f, int lg) {
 #pragma unroll
         for (int h = 0; h < KH; h++) {
             // (a NaN or an infinity times the zero marks a column that is NaN anyway)
@@ -87,26 +95,51 @@ struct Kv4Query {
                 od[h][i] *= mul;
                 m = max(m, max(__float_as_uint(ev[h][i]) & 0x7FFFFFFFu, __float_as_uint(od[h][i]) & 0x7FFFFFFFu));
             }
-            // the largest magnitude within (3.75, 7.5] of the first part's scale
-            int e = (int)(m >> 23) - 2 + ((m & 0x7FFFFFu) > 0x700000u);
-            e = min(max(e, 27), 252);
+            // the largest magnitude is at most 15/8 of the first part's scale
+            const int e = min(max((int)(m >> 23) + ((m & 0x7FFFFFu) > 0x700000u), 27), 254);
             const bool bad = m >= 0x7F800000u;
             scale[h][0] = bad ? 0xFFFFFFFFu : (uint32_t)(e | (e - 4) << 8 | (e - 8) << 16 | (e - 12) << 24);
             scale[h][1] = bad ? 0xFFFFFFFFu : (uint32_t)((e - 16) | (e - 20) << 8);
-#pragma unroll
-            for (int n = 0; n < kQParts; n++) {
-                const float s = __uint_as_float((uint32_t)(e - 4 * n) << 23);
-                part[h][n] = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(ev[h], od[h], s);
-                if (n + 1 < kQParts) {
-                    const f32x32 v = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(part[h][n], s);
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        ev[h][i] -= v[2 * i];
-                        od[h][i] -= v[2 * i + 1];
-                    }
-                }
-            }
         }
+    }
+
+    // Part n of half h: with T_n the nearest integer to 8 16^n q / s, the
+    // digit T_n - 16 T_(n - 1).  Any part by itself, so that the wavefronts of
+    // a workgroup can make one each: a conversion takes some 125 clocks.
+    __device__ __forceinline__ u32x6 digit(int h, int n) const {
+        const int e = (int)(scale[h][0] & 255);
+        const float f = __uint_as_float((uint32_t)(257 - e + 4 * n) << 23);
+        const float before = n ? __uint_as_float((uint32_t)(253 - e + 4 * n) << 23) : 0.f;
+        f32x16 a, b;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            a[i] = fmaf(-16.f, rintf(ev[h][i] * before), rintf(ev[h][i] * f));
+            b[i] = fmaf(-16.f, rintf(od[h][i] * before), rintf(od[h][i] * f));
+        }
+        return __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 8.0f);
+    }
+};
+
+// The parts of a tile's columns in LDS.
+template <int HD>
+struct Kv4SharedQuery {
+    static constexpr int KH = (HD + 127) / 128;
+    uint2 w[KH][kQParts][3][4][16];
+    __device__ __forceinline__ void put(const u32x6 &p, int h, int n, int r, int lg) {
+#pragma unroll
+        for (int i = 0; i < 3; i++) w[h][n][i][lg][r] = make_uint2(p[2 * i], p[2 * i + 1]);
+    }
+    __device__ __forceinline__ void get(Kv4Query<HD> &q, int r, int lg) const {
+#pragma unroll
+        for (int h = 0; h < KH; h++)
+#pragma unroll
+            for (int n = 0; n < kQParts; n++)
+#pragma unroll
+                for (int i = 0; i < 3; i++) {
+                    const uint2 x = w[h][n][i][lg][r];
+                    q.part[h][n][2 * i] = x.x;
+                    q.part[h][n][2 * i + 1] = x.y;
+                }
     }
 };
 
@@ -133,29 +166,34 @@ struct Kv4Key {
     }
 };
 
-template <int N, int HD>
-__device__ __forceinline__ void score_part(const i32x8 &k, uint32_t ks, const Kv4Query<HD> &q, int h, f32x4 &s) {
+// Part N's products of TILES tiles of 16 keys with 16 columns.
+template <int N, int HD, int TILES>
+__device__ __forceinline__ void score_part(const Kv4Key<HD> (&k)[TILES], const Kv4Query<HD> &q, int h, f32x4 (&s)[TILES]) {
     const u32x6 p = q.part[h][N];
     const i32x8 b = {(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)p[4], (int)p[5], 0, 0};
-    s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, b, s, 4 /* fp4 */, 2 /* fp6 e2m3 */, 0, (int)ks, N & 3,
-                                                         (int)q.scale[h][N >> 2]);
+#pragma unroll
+    for (int i = 0; i < TILES; i++) {
+        const u32x4 c = k[i].code[h];
+        const i32x8 a = {(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0};
+        s[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, s[i], 4 /* fp4 */, 2 /* fp6 e2m3 */, 0,
+                                                                (int)k[i].scale[h], N & 3, (int)q.scale[h][N >> 2]);
+    }
 }
 
-// Scores (log2 units) of 16 keys and 16 columns; the smallest parts first.
-template <int HD>
-__device__ __forceinline__ f32x4 kv4_scores(const Kv4Key<HD> &k, const Kv4Query<HD> &q) {
-    f32x4 s{0.f, 0.f, 0.f, 0.f};
+// Scores in log2 units, the smallest parts first.
+template <int HD, int TILES>
+__device__ __forceinline__ void kv4_scores(const Kv4Key<HD> (&k)[TILES], const Kv4Query<HD> &q, f32x4 (&s)[TILES]) {
+#pragma unroll
+    for (int i = 0; i < TILES; i++) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int h = 0; h < Kv4Key<HD>::KH; h++) {
-        const i32x8 a = {(int)k.code[h].x, (int)k.code[h].y, (int)k.code[h].z, (int)k.code[h].w, 0, 0, 0, 0};
-        score_part<5>(a, k.scale[h], q, h, s);
-        score_part<4>(a, k.scale[h], q, h, s);
-        score_part<3>(a, k.scale[h], q, h, s);
-        score_part<2>(a, k.scale[h], q, h, s);
-        score_part<1>(a, k.scale[h], q, h, s);
-        score_part<0>(a, k.scale[h], q, h, s);
+        score_part<5>(k, q, h, s);
+        score_part<4>(k, q, h, s);
+        score_part<3>(k, q, h, s);
+        score_part<2>(k, q, h, s);
+        score_part<1>(k, q, h, s);
+        score_part<0>(k, q, h, s);
     }
-    return s;
 }
 
 // A lane's HD / 16 dimensions of its eight keys of a unit of 32.
@@ -458,6 +496,7 @@ __global__ __launch_bounds__(64 * kv4_waves<HD>()) void kv4_attn_rows_kernel(con
     constexpr int SUMS = NW * 16 * PITCH, WEIGHTS = 16 * kKv4MaxRuns;
     __shared__ __attribute__((aligned(16))) float s_o[SUMS > WEIGHTS ? SUMS : WEIGHTS];
     __shared__ float s_m[16][NW], s_l[16][NW];
+    __shared__ Kv4SharedQuery<HD> s_q;
     __shared__ Kv4NewRow<HD> s_new;
     __shared__ unsigned s_arrived;
     __shared__ int s_first[ONE ? 1 : kKv4FlatItems + 1];  // the items' first blocks in the row of all
@@ -573,7 +612,8 @@ __global__ __launch_bounds__(64 * kv4_waves<HD>()) void kv4_attn_rows_kernel(con
         const int cols = it.cols, pos = it.pos;
         Kv4State<HD> st;
         if (pos >= 0) {
-            const int qpos = r < cols ? pos + it.t0 + div_group(a, it.h0 + r) : -1;
+            // (lanes past the columns repeat the last one)
+            const int qpos = pos + it.t0 + div_group(a, it.h0 + min(r, cols - 1));
             const int first_pos = pos + it.t0;
             int key0 = b * BLOCK + 32 * wave;
             const int end = min(bend * BLOCK, it.last + 1);
@@ -581,7 +621,16 @@ __global__ __launch_bounds__(64 * kv4_waves<HD>()) void kv4_attn_rows_kernel(con
                 fetch(it.seq, it.t0, it.h0, cols);
                 load(pl, key0, it.last);
             }
-            q.split(a.scale * 1.4426950408889634f, lg);
+            // the wavefronts make the query's parts together
+            q.ready(a.scale * 1.4426950408889634f, lg);
+#pragma unroll
+            for (int h = 0; h < Kv4Query<HD>::KH; h++)
+                for (int n = wave; n < kQParts; n += NW) {
+                    const u32x6 d = q.digit(h, n);
+                    if (r < cols) s_q.put(d, h, n, r, lg);
+                }
+            lds_barrier();  // the keys may still be on their way
+            s_q.get(q, min(r, cols - 1), lg);
             for (; key0 < end; key0 += step * BLOCK) {
                 if (append && key0 + 31 >= pos) {
                     s_new.put(xn, lane, pl, row0 + pos);
@@ -590,10 +639,11 @@ __global__ __launch_bounds__(64 * kv4_waves<HD>()) void kv4_attn_rows_kernel(con
                     __builtin_amdgcn_wave_barrier();
                     s_new.patch(k, v, pos - key0, r, lg);
                 }
-                f32x4 s[2] = {kv4_scores(k[0], q), kv4_scores(k[1], q)};
+                f32x4 s[2];
+                kv4_scores(k, q, s);
                 Kv4Values<HD> vn = v;
                 if (key0 + step * BLOCK < end) load(pl, key0 + step * BLOCK, it.last);
-                if (key0 + 31 > first_pos || cols < 16) {
+                if (key0 + 31 > first_pos) {
 #pragma unroll
                     for (int j = 0; j < 8; j++)
                         if (key0 + 16 * (j >> 2) + 4 * lg + (j & 3) > qpos) s[j >> 2][j & 3] = -INFINITY;

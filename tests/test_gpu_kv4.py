@@ -117,8 +117,10 @@ def attend(c, q, pos, dev=None, new=None, q_stride=0, out_stride=0, new_stride=0
     return body[:, :width].reshape(q.shape)
 
 
-def check_attn(c, got, q, pos, scale=None):
+def check_attn(c, got, q, pos, scale=None, only=None):
     for b, p in enumerate(pos):
+        if only is not None and b not in only:
+            continue
         if p < 0 or p + q.shape[1] > c.cap:
             assert (got[b] == 0).all()
             continue
@@ -244,6 +246,44 @@ def test_attn_longer_pieces(T, H, n, pos):
     c.fill(rng, pos + n)
     q = rng.standard_normal((1, n, 2, 128)).astype(np.float32)
     check_attn(c, attend(c, q, [pos]), q, [pos])
+
+
+@pytest.mark.parametrize("hd,group,n", [(16, 2, 33), (32, 3, 45), (64, 4, 9), (64, 2, 100), (128, 2, 17), (128, 2, 100),
+                                        (128, 4, 40), (128, 8, 16), (128, 1, 129), (256, 2, 20), (256, 4, 33)])
+def test_attn_prompts_of_many_sequences(T, H, hd, group, n):
+    """Enough tiles of columns for the prompts' kernel: first pieces and later
+    ones, one column past a tile, idle slots, values and keys that are not
+    finite, strided rows."""
+    rng = np.random.default_rng(hd + group + n)
+    c = Cache(T, H, n + 150, 4, hd, n_seq=64, gap=32)
+
+    def spoil(k, at):
+        k[5, at, 1, hd // 2] = np.nan
+        k[7, at + 60, 0, 0] = np.inf
+        return k
+    c.fill(rng, n + 140, keys=lambda k: spoil(k, 61), values=lambda v: spoil(v, 63))
+    pos = [int(x) for x in rng.integers(0, 140, 64)]
+    pos[0], pos[1], pos[2], pos[3], pos[4], pos[5], pos[7] = 0, 150, -1, 151, 64, 40, 61
+    q = rng.standard_normal((64, n, 4 * group, hd)).astype(np.float32)
+    w = 4 * group * hd
+    got = attend(c, q, pos, dev=ints(H, pos), q_stride=w + 4, out_stride=w + 12)
+    check_attn(c, got, q, pos, only=(0, 1, 2, 3, 4, 5, 7, 8, 63))
+    # appended first: the same rows as written by themselves
+    new = rows(rng, c, n), rows(rng, c, n)
+    got = attend(c, q, pos, dev=ints(H, pos), new=new)
+    c.check()
+    check_attn(c, got, q, pos, only=(0, 3, 9))
+
+
+def test_attn_long_prompt(T, H):
+    """One sequence of more than 2048 rows."""
+    rng = np.random.default_rng(77)
+    c = Cache(T, H, 2200, 8, 128)
+    c.fill(rng, 2200)
+    q = rng.standard_normal((1, 2100, 16, 128)).astype(np.float32)
+    got = attend(c, q, [71])
+    for t in (0, 1, 63, 64, 1000, 2047, 2099):
+        check_attn(c, got[:, t:t + 1], q[:, t:t + 1], [71 + t])
 
 
 def test_attn_sharp_and_flat_softmax(T, H):

@@ -16,7 +16,7 @@
 // Values.  A value's scale belongs to a (position, 32 dimensions), which the
 // instruction cannot take along its contracted axis, so values are widened to
 // bf16 (exact) and multiplied on the bf16 MFMA with P as three bf16 parts
-// (2^-26 of a probability left out).
+// (exact).
 //
 // Layouts (lane l: r = l & 15, lg = l >> 4).  S^T = K Q^T: lane (r, lg)
 // supplies dims 32 lg .. +31 of key r and of column r, and receives keys
@@ -118,6 +118,23 @@ struct Kv4Query {
         }
         return __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 8.0f);
     }
+
+    // The parts of half h one after the other: n = 0, 1, ..  What they leave
+    // stays in ev and od.
+    __device__ __forceinline__ u32x6 next_digit(int h, int n) {
+        const int e = (int)(scale[h][0] & 255);
+        const float f = __uint_as_float((uint32_t)(257 - e + 4 * n) << 23);
+        const float back = -__uint_as_float((uint32_t)(e - 3 - 4 * n) << 23);
+        f32x16 a, b;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            a[i] = rintf(ev[h][i] * f);
+            b[i] = rintf(od[h][i] * f);
+            ev[h][i] = fmaf(a[i], back, ev[h][i]);
+            od[h][i] = fmaf(b[i], back, od[h][i]);
+        }
+        return __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 8.0f);
+    }
 };
 
 // The parts of a tile's columns in LDS.
@@ -180,19 +197,21 @@ __device__ __forceinline__ void score_part(const Kv4Key<HD> (&k)[TILES], const K
     }
 }
 
-// Scores in log2 units, the smallest parts first.
+// Scores in log2 units, less `ref`: the sums start from -ref and the largest
+// part, so that what follows is added to numbers as small as the differences.
 template <int HD, int TILES>
-__device__ __forceinline__ void kv4_scores(const Kv4Key<HD> (&k)[TILES], const Kv4Query<HD> &q, f32x4 (&s)[TILES]) {
+__device__ __forceinline__ void kv4_scores(const Kv4Key<HD> (&k)[TILES], const Kv4Query<HD> &q, float ref, f32x4 (&s)[TILES]) {
 #pragma unroll
-    for (int i = 0; i < TILES; i++) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < TILES; i++) s[i] = f32x4{-ref, -ref, -ref, -ref};
+#pragma unroll
+    for (int h = 0; h < Kv4Key<HD>::KH; h++) score_part<0>(k, q, h, s);
 #pragma unroll
     for (int h = 0; h < Kv4Key<HD>::KH; h++) {
-        score_part<5>(k, q, h, s);
-        score_part<4>(k, q, h, s);
-        score_part<3>(k, q, h, s);
-        score_part<2>(k, q, h, s);
         score_part<1>(k, q, h, s);
-        score_part<0>(k, q, h, s);
+        score_part<2>(k, q, h, s);
+        score_part<3>(k, q, h, s);
+        score_part<4>(k, q, h, s);
+        score_part<5>(k, q, h, s);
     }
 }
 
@@ -262,20 +281,28 @@ struct Kv4Values {
     }
 };
 
-// P as bf16 parts, each what the ones before leave.
-template <int PARTS>
-__device__ __forceinline__ void split_p(const float (&p)[8], bf16x8 (&out)[PARTS]) {
-    float rest[8];
+// Eight weights as three bf16 parts, their upper, middle and lower eight
+// significant bits: exact.
+__device__ __forceinline__ void split_p(const float *p, bf16x8 (&out)[3]) {
+    uint32_t hi[8], mid[8], lo[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) rest[j] = p[j];
-#pragma unroll
-    for (int n = 0; n < PARTS; n++) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            out[n][j] = (__bf16)rest[j];
-            rest[j] -= (float)out[n][j];
-        }
+    for (int j = 0; j < 8; j++) {
+        hi[j] = __float_as_uint(p[j]) & 0xFFFF0000u;
+        const float m = p[j] - __uint_as_float(hi[j]);
+        mid[j] = __float_as_uint(m);
+        lo[j] = __float_as_uint(m - __uint_as_float(mid[j] & 0xFFFF0000u));
     }
+    u32x4 a, b, c;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        // the upper halves of two words
+        a[j] = __builtin_amdgcn_perm(hi[2 * j + 1], hi[2 * j], 0x07060302u);
+        b[j] = __builtin_amdgcn_perm(mid[2 * j + 1], mid[2 * j], 0x07060302u);
+        c[j] = __builtin_amdgcn_perm(lo[2 * j + 1], lo[2 * j], 0x07060302u);
+    }
+    out[0] = __builtin_bit_cast(bf16x8, a);
+    out[1] = __builtin_bit_cast(bf16x8, b);
+    out[2] = __builtin_bit_cast(bf16x8, c);
 }
 
 template <int PARTS>
@@ -321,43 +348,44 @@ __device__ __forceinline__ void nan_values(F marked, int key0, int qpos, int lg,
 // Running softmax state of a lane's column over the keys its wavefront took.
 template <int HD>
 struct Kv4State {
-    float m = -INFINITY, l = 0.f;
+    float ref = 0.f;   // what the weights are relative to
+    bool any = false;  // ref is a score's; before that, no score was above -inf
+    float l = 0.f;
     f32x4 o[HD / 16];
     __device__ Kv4State() {
 #pragma unroll
         for (int t = 0; t < HD / 16; t++) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    // The reference of a merge: -inf where no score was above it.
+    __device__ __forceinline__ float max_ref() const { return any ? ref : -INFINITY; }
 
-    // The scores of a unit's two key tiles become weights.  The maximum is
-    // raised in steps of at least 2^8 only: weights up to 2^8 cost no
-    // precision in f32, and most units then leave the sums as they are.
-    __device__ __forceinline__ void weights(const f32x4 (&s)[2], float (&p)[8]) {
-        float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
-        mx = fmaxf(mx, fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    // The scores of some key tiles, less ref, become weights.  The reference
+    // is raised in steps of at least 2^8 only: weights up to 2^8 cost no
+    // precision in f32, and most blocks then leave the sums as they are.
+    template <int TILES>
+    __device__ __forceinline__ void weights(f32x4 (&s)[TILES], float (&p)[4 * TILES]) {
+        float mx = s[0][0];
+#pragma unroll
+        for (int j = 1; j < 4 * TILES; j++) mx = fmaxf(mx, s[j >> 2][j & 3]);
         mx = max_xor16_32(mx);
-        const bool raise = mx > m + 8.0f;
+        const bool raise = any ? mx > 8.0f : mx > -INFINITY;
         if (__builtin_amdgcn_ballot_w64(raise)) {
-            const float corr = raise ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
-            m = raise ? mx : m;
+            const float up = raise ? mx : 0.0f, corr = raise ? (any ? __builtin_amdgcn_exp2f(-mx) : 0.0f) : 1.0f;
+            ref += up;
+            any |= raise;
             l *= corr;
 #pragma unroll
             for (int t = 0; t < HD / 16; t++) o[t] *= corr;
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            p[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3] - ref);
+            for (int j = 0; j < 4 * TILES; j++) s[j >> 2][j & 3] -= up;
+        }
+#pragma unroll
+        for (int j = 0; j < 4 * TILES; j++) {
+            p[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3]);
             l += p[j];
         }
     }
 };
-
-// An output element, as f32 or as the split-bf16 planes of a following GEMM.
-__device__ __forceinline__ void kv4_store(const Kv4AttnArgs &a, int seq, int row, int d, float v) {
-    const size_t i = ((size_t)seq * a.rows + row) * a.out_stride + d;
-    if (a.out) a.out[i] = v;
-    if (a.out_hi) split_bf16(v, a.out_hi + i, a.out_lo + i);
-}
 
 // A new row of one head, quantized by a wavefront, in LDS in the cache's layout.
 template <int HD>
@@ -462,10 +490,14 @@ __device__ __forceinline__ void kv4_put(const Kv4AttnArgs &a, const Kv4Item &it,
     if (a.out_hi) split_bf16(v, a.out_hi + i, a.out_lo + i);
 }
 
-// Wavefronts of a workgroup; a wavefront takes 32 keys of a block.
-template <int HD>
+// Wavefronts of a workgroup; a wavefront takes 32 keys of a block.  One item
+// alone is spread over eight (fewer workgroups to merge); of several, two
+// workgroups of four share a CU, so that one's loads, query and merge run
+// beside the other's products (48 ragged sequences: 44 us with one of eight).
+// At head dim 256 the registers leave room for one wavefront a SIMD.
+template <int HD, bool ONE>
 constexpr int kv4_waves() {
-    return HD == 256 ? 4 : 8;  // at 256 its registers leave room for one a SIMD
+    return ONE && HD < 256 ? 8 : 4;
 }
 
 // A workgroup owns one KV head and a run of blocks (32 keys a wavefront), each
@@ -490,8 +522,8 @@ constexpr int kv4_waves() {
 // Bound by the latency of its loads and of the merge for one sequence, by the
 // cache's bytes for many.
 template <int HD, bool ONE>
-__global__ __launch_bounds__(64 * kv4_waves<HD>()) void kv4_attn_rows_kernel(const Kv4AttnArgs a) {
-    constexpr int DPL = HD / 16, PITCH = HD + 4, NW = kv4_waves<HD>(), NT = 64 * NW, BLOCK = 32 * NW;
+__global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) void kv4_attn_rows_kernel(const Kv4AttnArgs a) {
+    constexpr int DPL = HD / 16, PITCH = HD + 4, NW = kv4_waves<HD, ONE>(), NT = 64 * NW, BLOCK = 32 * NW;
     // the wavefronts' sums [NW][16][PITCH], then the runs' weights [16][kKv4MaxRuns]
     constexpr int SUMS = NW * 16 * PITCH, WEIGHTS = 16 * kKv4MaxRuns;
     __shared__ __attribute__((aligned(16))) float s_o[SUMS > WEIGHTS ? SUMS : WEIGHTS];
@@ -577,7 +609,7 @@ __global__ __launch_bounds__(64 * kv4_waves<HD>()) void kv4_attn_rows_kernel(con
         __syncthreads();
         item = __builtin_amdgcn_readfirstlane(s_start);
     } else {
-        item = run;
+        item = a.items - 1 - run;  // the latest rows, with the most keys, first
     }
     const int x_begin = x;
     for (; x < xend; item++) {
@@ -640,7 +672,7 @@ __global__ __launch_bounds__(64 * kv4_waves<HD>()) void kv4_attn_rows_kernel(con
                     s_new.patch(k, v, pos - key0, r, lg);
                 }
                 f32x4 s[2];
-                kv4_scores(k, q, s);
+                kv4_scores(k, q, st.ref, s);
                 Kv4Values<HD> vn = v;
                 if (key0 + step * BLOCK < end) load(pl, key0 + step * BLOCK, it.last);
                 if (key0 + 31 > first_pos) {
@@ -668,7 +700,7 @@ __global__ __launch_bounds__(64 * kv4_waves<HD>()) void kv4_attn_rows_kernel(con
 #pragma unroll
                 for (int d = 0; d < DPL; d++) dst[i * DPL + d] = st.o[d][i];
             if (lg == 0) {
-                s_m[r][wave] = st.m;
+                s_m[r][wave] = st.max_ref();
                 s_l[r][wave] = st.l;
             }
         }
@@ -781,46 +813,294 @@ __global__ __launch_bounds__(64 * kv4_waves<HD>()) void kv4_attn_rows_kernel(con
     }
 }
 
+// ---- many columns -----------------------------------------------------------
+
+// Column tiles of 16 of a wavefront; a workgroup is four wavefronts.
+template <int HD>
+constexpr int kv4_col_tiles() {
+    return HD == 256 ? 1 : 2;
+}
+constexpr int kTileKeys = 64;  // keys of a block
+
+// A wavefront's share of widening a block's values: a unit of 32 keys, and
+// half of a lane's dimensions (all of them where a lane has one or two; then
+// only the even wavefronts have a share).
+template <int HD>
+struct Kv4Stage {
+    static constexpr int DPL = HD / 16, TILES = DPL < 4 ? DPL : DPL / 2;
+    uint32_t code[8], scale[8];
+
+    __device__ __forceinline__ void load(const uint8_t *vc, const uint8_t *vs, int d, int half, int r, int lg) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const unsigned row = (unsigned)min(16 * (j >> 2) + 4 * lg + (j & 3), d);
+            const uint8_t *p = vc + row * (HD / 2);
+            if constexpr (HD == 256)
+                code[j] = *reinterpret_cast<const uint32_t *>(p + 8 * r + 4 * half);
+            else if constexpr (HD == 128)
+                code[j] = *reinterpret_cast<const uint16_t *>(p + 4 * r + 2 * half);
+            else if constexpr (HD == 64)
+                code[j] = p[2 * r + half];
+            else
+                code[j] = p[HD == 32 ? r : r >> 1];
+            scale[j] = vs[row * kv4_groups(HD) + r * DPL / 32];
+        }
+    }
+
+    // The tiles' bf16 operands to dst[tile][64 lanes]; the marked lanes of
+    // each key to mark, and whether there are any to *any (by half 0).
+    __device__ __forceinline__ void store(u32x4 (*dst)[64], unsigned long long *mark, int *any, int half, int lane) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (scale[j] == kKv4BadScale) {
+                bad |= 1u << j;
+                scale[j] = 127;
+            }
+        const bool some = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+        if (half == 0) {
+            if (some) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const unsigned long long lanes = __builtin_amdgcn_ballot_w64((bad >> j) & 1);
+                    if (lane == 0) mark[j] = lanes;
+                }
+            }
+            if (lane == 0) *any = some;
+        }
+        put<0>(dst + (DPL < 4 ? 0 : half * TILES), lane);
+    }
+
+  private:
+    template <int I>
+    __device__ __forceinline__ void put(u32x4 (*dst)[64], int lane) const {
+        if constexpr (2 * I < TILES) {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                w[j] = __builtin_bit_cast(
+                    uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(code[j], kv4_scale(scale[j]), I));
+            const uint32_t pick = HD == 16 && (lane & 1) ? 0x07060302u : 0x05040100u;
+            u32x4 even, odd;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                even[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], pick);
+                odd[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);
+            }
+            dst[2 * I][lane] = even;
+            if constexpr (2 * I + 1 < TILES) dst[2 * I + 1][lane] = odd;
+            put<I + 1>(dst, lane);
+        }
+    }
+};
+
+// Long prompts: a workgroup owns a tile of 64 kv4_col_tiles() columns, 16
+// kv4_col_tiles() a wavefront, and goes through their blocks of 64 keys.  The
+// wavefronts read the block's keys straight into matrix operands; the values
+// are widened once for all of them, a share each, into LDS in operand order (a
+// lane's operand is 16 bytes at 16 lane: no bank conflicts), a block ahead.
+//
+// Workgroups of the latest positions come first: they have the most keys.
+// Bound by the MFMA and VALU issue of its two wavefronts a SIMD.
+template <int HD>
+__global__ __launch_bounds__(kBlock, 2) void kv4_attn_tile_kernel(const Kv4AttnArgs a) {
+    constexpr int DPL = HD / 16, CT = kv4_col_tiles<HD>(), TC = 64 * CT;
+    // the wavefronts' query parts at first, then the values of two blocks
+    constexpr size_t PARTS = 4 * sizeof(Kv4SharedQuery<HD>), VALUES = 4 * DPL * 64 * sizeof(u32x4);
+    __shared__ __attribute__((aligned(16))) char s_buf[PARTS > VALUES ? PARTS : VALUES];
+    Kv4SharedQuery<HD> *const s_q = reinterpret_cast<Kv4SharedQuery<HD> *>(s_buf);
+    u32x4 (*const s_v)[2][DPL][64] = reinterpret_cast<u32x4 (*)[2][DPL][64]>(s_buf);
+    __shared__ unsigned long long s_mark[2][2][8];
+    __shared__ int s_any[2][2];
+    const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r = lane & 15, lg = lane >> 4;
+    const int g = (int)(blockIdx.x % (unsigned)a.c.nkv);
+    const unsigned rest = blockIdx.x / (unsigned)a.c.nkv;
+    const int seq = (int)(rest % (unsigned)a.c.n_seq), tile = a.ntile - 1 - (int)(rest / (unsigned)a.c.n_seq);
+    const int ncol = a.rows * a.group, cols = min(TC, ncol - TC * tile);
+    const int pos = kv4_pos(a.pos_dev, a.pos, seq, a.rows, a.c.cap);
+    const int t0 = TC * tile / a.group, h0 = TC * tile - t0 * a.group;
+    const int last = pos + t0 + div_group(a, h0 + cols - 1);
+    const int nb = pos < 0 ? 0 : last / kTileKeys + 1;
+    const Kv4Planes<HD> pl(a.c, seq);
+    const size_t row0 = (size_t)g * a.c.cap;
+
+    int col[CT], qpos[CT];  // in the tile; lanes past the columns repeat the last one
+    Kv4Query<HD> q[CT];
+    Kv4State<HD> st[CT];
+    const bool mine = 16 * CT * wave < cols;
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        col[c] = 16 * (CT * wave + c) + r;
+        const int dt = div_group(a, h0 + min(col[c], cols - 1)), h = h0 + min(col[c], cols - 1) - dt * a.group;
+        qpos[c] = pos + t0 + dt;
+        q[c].fetch(a.q + ((size_t)seq * a.rows + t0 + dt) * a.q_stride + (size_t)(g * a.group + h) * HD, lg);
+    }
+    const int wave_first = pos + t0 + div_group(a, h0 + min(16 * CT * wave, cols - 1));
+    const int wave_last = pos + t0 + div_group(a, h0 + min(16 * CT * (wave + 1), cols) - 1);
+    const int unit = wave >> 1, half = wave & 1;
+    const bool stages = DPL >= 4 || half == 0;
+
+    Kv4Key<HD> k[4];
+    Kv4Stage<HD> v;
+    auto load_keys = [&](int key0) {
+        const int at = min(key0, last), d = last - at;
+        const size_t row = row0 + at;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            k[i].load(pl.kc + row * (HD / 2), pl.ks + row * kv4_groups(HD), (unsigned)min(16 * i + r, d), lg);
+    };
+    auto load_values = [&](int key0) {
+        const int at = min(key0 + 32 * unit, last);
+        const size_t row = row0 + at;
+        v.load(pl.vc + row * (HD / 2), pl.vs + row * kv4_groups(HD), last - at, half, r, lg);
+    };
+    if (nb) {
+        load_keys(0);
+        if (stages) load_values(0);
+    }
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        q[c].ready(a.scale * 1.4426950408889634f, lg);
+        // through LDS, so that the parts are made in a loop: unrolled they
+        // are most of the kernel's code
+#pragma unroll
+        for (int h = 0; h < Kv4Query<HD>::KH; h++)
+#pragma unroll 1
+            for (int n = 0; n < kQParts; n++) s_q[wave].put(q[c].next_digit(h, n), h, n, r, lg);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        s_q[wave].get(q[c], r, lg);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    lds_barrier();  // the values take the parts' place
+    if (nb && stages) {
+        v.store(s_v[0][unit], s_mark[0][unit], &s_any[0][unit], half, lane);
+        load_values(kTileKeys);
+    }
+    lds_barrier();
+    for (int b = 0; b < nb; b++) {
+        const int key0 = b * kTileKeys, buf = b & 1;
+        const bool work = mine && key0 <= wave_last;
+        bf16x8 p[CT][2][3];
+        if (work) {
+            f32x4 s[CT][4];
+#pragma unroll
+            for (int c = 0; c < CT; c++) kv4_scores(k, q[c], st[c].ref, s[c]);
+            load_keys(key0 + kTileKeys);
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                if (key0 + kTileKeys - 1 > wave_first) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        if (key0 + 16 * (j >> 2) + 4 * lg + (j & 3) > qpos[c]) s[c][j >> 2][j & 3] = -INFINITY;
+                }
+                float w[16];
+                st[c].weights(s[c], w);
+                split_p(w, p[c][0]);
+                split_p(w + 8, p[c][1]);
+            }
+        }
+        // the next block's values, while this one's are multiplied
+        if (b + 1 < nb && stages) {
+            v.store(s_v[buf ^ 1][unit], s_mark[buf ^ 1][unit], &s_any[buf ^ 1][unit], half, lane);
+            load_values(key0 + 2 * kTileKeys);
+        }
+        if (work) {
+#pragma unroll
+            for (int d = 0; d < DPL; d++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const u32x4 x = s_v[buf][u][d][lane];
+#pragma unroll
+                    for (int c = 0; c < CT; c++) st[c].o[d] = mfma_pv(x, p[c][u], st[c].o[d]);
+                }
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (s_any[buf][u])
+#pragma unroll
+                    for (int c = 0; c < CT; c++)
+                        nan_values<HD>([&](int j) { return s_mark[buf][u][j]; }, key0 + 32 * u, qpos[c], lg, st[c].o);
+        }
+        lds_barrier();
+    }
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        const float l = add_xor32(add_xor16(st[c].l)), f = l == 0.f ? 0.f : 1.0f / l;
+        if (col[c] >= cols) continue;
+        const int dt = div_group(a, h0 + col[c]), h = h0 + col[c] - dt * a.group;
+        const size_t to = ((size_t)seq * a.rows + t0 + dt) * a.out_stride + (size_t)(g * a.group + h) * HD;
+        constexpr int VEC = DPL < 4 ? DPL : 4;
+        typedef float vec __attribute__((ext_vector_type(VEC)));
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int d = 0; d < DPL; d += VEC) {
+                const size_t at = to + (4 * lg + i) * DPL + d;
+                vec y;
+#pragma unroll
+                for (int e = 0; e < VEC; e++) y[e] = st[c].o[d + e][i] * f;
+                if (a.out) *reinterpret_cast<vec *>(a.out + at) = y;
+                if (a.out_hi)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) split_bf16(y[e], a.out_hi + at + e, a.out_lo + at + e);
+            }
+    }
+}
+
 }  // namespace
 
 Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq) {
     Kv4Plan p{};
     const int64_t ncol = (int64_t)rows * (nq / c.nkv);
+    const int tc = 64 * (c.hd == 256 ? kv4_col_tiles<256>() : kv4_col_tiles<128>());
+    p.ntile = (int)((ncol + tc - 1) / tc);
+    p.items = (int64_t)p.ntile * c.n_seq;
+    p.runs = 1;
+    p.tile = ncol > kKv4RowCols && p.items * c.nkv >= kKv4TileWorkgroups;
+    if (p.tile) return p;
     p.part_cols = (int)std::min<int64_t>(16, ncol);
-    p.items = (ncol + 15) / 16 * c.n_seq;
-    const int block = c.hd == 256 ? 32 * kv4_waves<256>() : 32 * kv4_waves<128>();
+    p.ntile = (int)((ncol + 15) / 16);
+    p.items = (int64_t)p.ntile * c.n_seq;
+    const bool one = p.items == 1;
+    const int block = one && c.hd < 256 ? 32 * kv4_waves<128, true>() : 32 * kv4_waves<128, false>();
     const int64_t nb = ((int64_t)c.cap + block - 1) / block;
-    p.flat = p.items > 1 && p.items <= kKv4FlatItems && p.items * nb <= 1 << 30;
-    if (p.items > 1 && !p.flat) {
-        p.runs = (int)std::min<int64_t>(p.items, 0x7fffffff);
-    } else {
-        p.runs = (int)std::min<int64_t>({kKv4MaxRuns, p.items * nb, std::max(1, kKv4Workgroups / c.nkv)});
+    const int groups = one && c.hd < 256 ? kKv4Workgroups / 2 : kKv4Workgroups;
+    p.flat = !one && p.items * c.nkv <= kKv4Workgroups && p.items * nb <= 1 << 30;
+    if (one || p.flat) {
+        p.runs = (int)std::min<int64_t>({kKv4MaxRuns, p.items * nb, std::max(1, groups / c.nkv)});
         p.split = nb > 1 && p.runs > 1;
+    } else {
+        p.runs = (int)std::min<int64_t>(p.items, 0x7fffffff);
     }
     return p;
 }
 
+// Partial states of a launch: a run has two slots.
+static size_t kv4_part_states(const Kv4Plan &p, int nkv) { return p.split ? (size_t)2 * nkv * p.runs * p.part_cols : 0; }
+
 size_t kv4_attn_ws_bytes(const Kv4Cache &c, int rows, int nq) {
-    const Kv4Plan p = plan_kv4_attn(c, rows, nq);
-    return p.split ? kKv4CounterBytes + (size_t)2 * c.nkv * p.runs * p.part_cols * (c.hd + 2) * 4 : 0;
+    const size_t n = kv4_part_states(plan_kv4_attn(c, rows, nq), c.nkv);
+    return n ? kKv4CounterBytes + n * (c.hd + 2) * 4 : 0;
 }
 
 namespace {
 
 template <int HD>
-void launch_rows(const Kv4AttnArgs &a, unsigned grid, hipStream_t s) {
-    const dim3 block(64 * kv4_waves<HD>());
-    if (a.items == 1)
-        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, true>), dim3(grid), block, 0, s, a);
+void launch_attn_hd(const Kv4AttnArgs &a, bool tile, unsigned grid, hipStream_t s) {
+    if (tile)
+        hipLaunchKernelGGL((kv4_attn_tile_kernel<HD>), dim3(grid), dim3(kBlock), 0, s, a);
+    else if (a.items == 1)
+        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, true>), dim3(grid), dim3(64 * kv4_waves<HD, true>()), 0, s, a);
     else
-        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, false>), dim3(grid), block, 0, s, a);
+        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, false>), dim3(grid), dim3(64 * kv4_waves<HD, false>()), 0, s, a);
 }
 
 }  // namespace
 
 hipError_t launch_kv4_attn(Kv4AttnArgs a, void *ws, hipStream_t s) {
     const Kv4Plan p = plan_kv4_attn(a.c, a.rows, a.nq);
-    const int64_t grid = (int64_t)p.runs * a.c.nkv;
+    const int64_t grid = (p.tile ? p.items : 1) * p.runs * a.c.nkv;
     if (grid > 0x7fffffff || (p.split && !ws)) return hipErrorInvalidValue;
     if (a.k_new && a.rows > 1) {
         const Kv4WriteArgs w{a.c, a.k_new, a.v_new, a.new_stride, a.rows, a.pos_dev, a.pos};
@@ -830,20 +1110,20 @@ hipError_t launch_kv4_attn(Kv4AttnArgs a, void *ws, hipStream_t s) {
     }
     a.group = a.nq / a.c.nkv;
     a.inv_group = 1.0f / (float)a.group;
-    a.ntile = (a.rows * a.group + 15) / 16;
+    a.ntile = p.ntile;
     a.items = (int)p.items;
     a.flat = p.flat;
     a.runs = p.runs;
     a.part_cols = p.part_cols;
     a.arrived = (unsigned *)ws;
-    a.part_ml = (float *)((char *)ws + kKv4CounterBytes);
-    a.part = a.part_ml + (size_t)2 * grid * p.part_cols * 2;
+    a.part = (float *)((char *)ws + kKv4CounterBytes);
+    a.part_ml = a.part + kv4_part_states(p, a.c.nkv) * a.c.hd;
     switch (a.c.hd) {
-        case 16: launch_rows<16>(a, (unsigned)grid, s); break;
-        case 32: launch_rows<32>(a, (unsigned)grid, s); break;
-        case 64: launch_rows<64>(a, (unsigned)grid, s); break;
-        case 128: launch_rows<128>(a, (unsigned)grid, s); break;
-        case 256: launch_rows<256>(a, (unsigned)grid, s); break;
+        case 16: launch_attn_hd<16>(a, p.tile, (unsigned)grid, s); break;
+        case 32: launch_attn_hd<32>(a, p.tile, (unsigned)grid, s); break;
+        case 64: launch_attn_hd<64>(a, p.tile, (unsigned)grid, s); break;
+        case 128: launch_attn_hd<128>(a, p.tile, (unsigned)grid, s); break;
+        case 256: launch_attn_hd<256>(a, p.tile, (unsigned)grid, s); break;
         default: return hipErrorInvalidValue;
     }
     return hipGetLastError();

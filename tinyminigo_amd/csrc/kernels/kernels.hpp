@@ -415,19 +415,27 @@ struct Kv4AttnArgs {
     unsigned *arrived;
     float *part, *part_ml;
 };
-constexpr int kKv4Workgroups = 256;   // of 512 threads: one per CU
+constexpr int kKv4Workgroups = 512;   // of 256 threads: two per CU
 constexpr int kKv4MaxRuns = 256;
-constexpr int kKv4FlatItems = 1024;   // more items than this are a workgroup each
+// Most items cut into equal runs: more of them, times the KV heads, than
+// kKv4Workgroups are a workgroup each.
+constexpr int kKv4FlatItems = kKv4Workgroups;
 constexpr int kKv4WholeBlocks = 2;    // blocks that one workgroup takes rather than share
 // Counters of the shared items, one a workgroup at most, at the start of the
 // workspace.
 constexpr size_t kKv4CounterBytes = kKv4Workgroups * 4;
+// More columns (query rows x heads of a KV head) of a sequence than kKv4RowCols
+// take the tile kernel, where its tiles are enough workgroups to fill the chip.
+constexpr int kKv4RowCols = 32;
+constexpr int64_t kKv4TileWorkgroups = 256;
 struct Kv4Plan {
-    int part_cols;  // columns (query rows x heads of a KV head) of an item's partial states
-    int64_t items;  // tiles of 16 columns of all sequences
-    int runs;       // workgroups of a KV head
-    bool flat;      // the items' blocks are cut into equal runs
-    bool split;     // an item may be shared by several workgroups
+    bool tile;      // the tile kernel, else the rows kernel
+    int part_cols;  // columns of an item's partial states
+    int ntile;      // column tiles of a sequence
+    int64_t items;  // column tiles of all sequences
+    int runs;       // rows kernel: workgroups of a KV head
+    bool flat;      // rows kernel: the items' blocks are cut into equal runs
+    bool split;     // rows kernel: an item may be shared by several workgroups
 };
 Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq);
 // Workspace enough for every position: counters, which are zero between

@@ -123,6 +123,14 @@ int tmg_model_config(const tmg_model *model, tmg_config *out);
  * max_pos rows per layer: f32 keys and values, [pos, n_kv*head_dim] per
  * layer, like the reference's flat per-layer Vec<f32>. */
 int tmg_cache_new(tmg_model *model, uint32_t max_pos, tmg_cache **out);
+/* The same with 4-bit keys and values (the format: tmg_kv4 below), at
+ * head_dim 128 a 7.5th of the f32 cache's memory and traffic.  No counterpart
+ * in the reference.  forward_token, forward_seq, prefill and decode_greedy
+ * quantize each position's rows as they are written, and the attention reads
+ * what the codes stand for, its own position's too; everything else of the
+ * model is as with an f32 cache, and so are len, reset and read (which gives
+ * what the codes stand for). */
+int tmg_cache_new_kv4(tmg_model *model, uint32_t max_pos, tmg_cache **out);
 void tmg_cache_free(tmg_cache *cache);
 /* KvCache::len(layer) (src/model.rs:283-285). */
 int tmg_cache_len(const tmg_cache *cache, uint32_t layer, uint32_t *len);
@@ -153,6 +161,12 @@ int tmg_prefill(tmg_model *model, tmg_cache *cache, const uint32_t *tokens, size
 int tmg_generate(tmg_model *model, const uint32_t *prompt, size_t n_prompt, const tmg_gen_params *params,
                  tmg_on_token_fn on_token, void *user, uint32_t *out_tokens, size_t out_cap, size_t *n_out,
                  float *first_logits, float *prefill_secs);
+
+/* tmg_generate over a 4-bit cache (tmg_cache_new_kv4).  No counterpart in the
+ * reference. */
+int tmg_generate_kv4(tmg_model *model, const uint32_t *prompt, size_t n_prompt, const tmg_gen_params *params,
+                     tmg_on_token_fn on_token, void *user, uint32_t *out_tokens, size_t out_cap, size_t *n_out,
+                     float *first_logits, float *prefill_secs);
 
 /* Greedy generation for n_seq independent prompts in one batch (1..128
  * sequences).  No counterpart in the reference, which decodes one sequence
@@ -239,7 +253,7 @@ int tmg_quantize_i8(const uint16_t *w_dev, uint32_t rows, uint32_t in, int8_t *q
  * 7 s, within [2^-100, 2^125], stored as the byte log2(s) + 127.  A code is
  * x / s rounded to the nearest magnitude, halves to the even code, magnitudes
  * above 6 to 6.  A group that holds an infinity or a NaN has the byte 255 and
- * reads back as NaN.
+ * reads back as NaN (253 and 254, which nothing writes, count as 255).
  *
  * A sequence's cache of `cap` positions is a slab of tmg_kv4_bytes(cap, nkv,
  * hd) DEVICE bytes, four planes one after the other: key codes
@@ -377,8 +391,8 @@ typedef struct tmg_floor_record {
  * chain per replay, one record per kind gives its phases back to back, and
  * *empty_ms is one empty 256-workgroup launch in a graph.  Needs 9 free
  * cache rows past the length; leaves the cache as it was.  Allocates the
- * slab (about the step's bytes) for the call.  No counterpart in the
- * reference (measurement only). */
+ * slab (about the step's bytes) for the call.  4-bit caches are rejected
+ * (TMG_E_INVALID).  No counterpart in the reference (measurement only). */
 int tmg_profile_step_floor(tmg_model *model, tmg_cache *cache, uint32_t token, tmg_floor_record *records,
                            size_t cap, size_t *n_records, float *step_ms, float *floor_ms, float *empty_ms);
 

@@ -217,6 +217,29 @@ def test_attn_single_token(T, H, ctx):
     check_attn(c, attend(c, q, [ctx - 1]), q, [ctx - 1])
 
 
+@pytest.mark.parametrize("hd", [16, 64, 128, 256])
+@pytest.mark.parametrize("fill", [0xFD, 0xFE, 0x7F, None])
+def test_attn_never_uses_unwritten_rows(T, H, hd, fill):
+    """Whatever the memory held: any scale byte, any code."""
+    rng = np.random.default_rng(hd)
+    c = Cache(T, H, 300, 2, hd, n_seq=2)
+    raw = rng.integers(0, 256, c.buf.nbytes, np.uint8) if fill is None else np.full(c.buf.nbytes, fill, np.uint8)
+    for ctx, n in ((1, 1), (20, 3), (140, 1), (200, 40)):
+        H.copy_device(c.buf, H.DeviceBuffer.from_array(raw), raw.size)
+        one = T.Kv4(c.buf.addr, cap=300, nkv=2, hd=hd)
+        for kv, seqs in ((one, 1), (c.kv, 2)):
+            c.n_seq, kept = seqs, c.kv
+            c.kv = kv
+            c.want[:] = np.nan
+            k, v = c.fill(rng, ctx)
+            q = rng.standard_normal((seqs, n, 4, hd)).astype(np.float32)
+            pos = [ctx - n] * seqs
+            check_attn(c, attend(c, q, pos), q, pos)
+            new = rows(rng, c, 1), rows(rng, c, 1)
+            check_attn(c, attend(c, q[:, :1], [ctx] * seqs, new=new), q[:, :1], [ctx] * seqs)
+            c.kv = kept
+
+
 @pytest.mark.parametrize("nkv,hd", HEADS)
 @pytest.mark.parametrize("group", [1, 2, 3, 4, 8, 20])
 def test_attn_head_layouts(T, H, nkv, hd, group):

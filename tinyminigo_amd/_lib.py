@@ -124,6 +124,7 @@ SIGNATURES = {
     "tmg_model_free": (None, [P]),
     "tmg_model_config": (C.c_int, [P, C.POINTER(tmg_config)]),
     "tmg_cache_new": (C.c_int, [P, C.c_uint32, C.POINTER(P)]),
+    "tmg_cache_new_kv4": (C.c_int, [P, C.c_uint32, C.POINTER(P)]),
     "tmg_cache_free": (None, [P]),
     "tmg_cache_len": (C.c_int, [P, C.c_uint32, PU32]),
     "tmg_cache_reset": (C.c_int, [P]),
@@ -132,6 +133,11 @@ SIGNATURES = {
     "tmg_forward_seq": (C.c_int, [P, P, PU32, C.c_size_t, PF]),
     "tmg_prefill": (C.c_int, [P, P, PU32, C.c_size_t, PF]),
     "tmg_generate": (
+        C.c_int,
+        [P, PU32, C.c_size_t, C.POINTER(tmg_gen_params), ON_TOKEN, P, PU32, C.c_size_t,
+         C.POINTER(C.c_size_t), PF, PF],
+    ),
+    "tmg_generate_kv4": (
         C.c_int,
         [P, PU32, C.c_size_t, C.POINTER(tmg_gen_params), ON_TOKEN, P, PU32, C.c_size_t,
          C.POINTER(C.c_size_t), PF, PF],

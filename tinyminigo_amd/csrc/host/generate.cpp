@@ -43,9 +43,9 @@ using namespace tmg;
         if (e_ != hipSuccess) return set_error(TMG_E_DEVICE, std::string("HIP error ") + hipGetErrorString(e_) + " in " #expr); \
     } while (0)
 
-extern "C" int tmg_generate(tmg_model *m, const uint32_t *prompt, size_t n_prompt, const tmg_gen_params *p,
-                            tmg_on_token_fn on_token, void *user, uint32_t *out_tokens, size_t out_cap, size_t *n_out,
-                            float *first_logits, float *prefill_secs) {
+static int generate(tmg_model *m, bool kv4, const uint32_t *prompt, size_t n_prompt, const tmg_gen_params *p,
+                    tmg_on_token_fn on_token, void *user, uint32_t *out_tokens, size_t out_cap, size_t *n_out,
+                    float *first_logits, float *prefill_secs) {
     clear_error();
     if (n_out) *n_out = 0;
     if (!m || !p || (!prompt && n_prompt)) return set_error(TMG_E_INVALID, "bad argument to tmg_generate");
@@ -73,7 +73,7 @@ extern "C" int tmg_generate(tmg_model *m, const uint32_t *prompt, size_t n_promp
     CacheGuard cg;
     const size_t max_pos = n_prompt + (size_t)p->max_tokens + 1;
     if (max_pos > 0x7fffffff) return set_error(TMG_E_INVALID, "sequence too long");
-    int rc = tmg_cache_new(m, (uint32_t)max_pos, &cg.c);
+    int rc = cache_new(m, (uint32_t)max_pos, kv4, &cg.c);
     if (rc) return rc;
     tmg_cache *c = cg.c;
 
@@ -148,4 +148,16 @@ extern "C" int tmg_generate(tmg_model *m, const uint32_t *prompt, size_t n_promp
     TMG_HIPG(hipStreamSynchronize(m->stream));
     if (n_out) *n_out = produced;
     return TMG_OK;
+}
+
+extern "C" int tmg_generate(tmg_model *m, const uint32_t *prompt, size_t n_prompt, const tmg_gen_params *p,
+                            tmg_on_token_fn on_token, void *user, uint32_t *out_tokens, size_t out_cap, size_t *n_out,
+                            float *first_logits, float *prefill_secs) {
+    return generate(m, false, prompt, n_prompt, p, on_token, user, out_tokens, out_cap, n_out, first_logits, prefill_secs);
+}
+
+extern "C" int tmg_generate_kv4(tmg_model *m, const uint32_t *prompt, size_t n_prompt, const tmg_gen_params *p,
+                                tmg_on_token_fn on_token, void *user, uint32_t *out_tokens, size_t out_cap,
+                                size_t *n_out, float *first_logits, float *prefill_secs) {
+    return generate(m, true, prompt, n_prompt, p, on_token, user, out_tokens, out_cap, n_out, first_logits, prefill_secs);
 }

@@ -416,6 +416,28 @@ static bool fused_merge(const tmg_model *m, const tmg_cache *c) {
     return c->attn_nsplit > 1 && c->attn_nsplit <= kFusedSplits && m->qd <= 4096;
 }
 
+Kv4Cache kv4_layer(const tmg_cache *c, int layer) {
+    const tmg_model *m = c->model;
+    return Kv4Cache{c->kv4 + (size_t)layer * kv4_slab_bytes(c->max_pos, m->nkv, m->hd), 0, 1, c->max_pos, m->nkv, m->hd};
+}
+
+// What the attention of one sequence's rows in a 4-bit cache takes, output
+// apart: the rows' keys and values are k and v [rows][kvd], appended first.
+static Kv4AttnArgs kv4_args(const tmg_model *m, const tmg_cache *c, int layer, const float *q, const float *k,
+                            const float *v, int rows) {
+    Kv4AttnArgs a{};
+    a.c = kv4_layer(c, layer);
+    a.q = q;
+    a.q_stride = a.out_stride = m->qd;
+    a.k_new = k;
+    a.v_new = v;
+    a.new_stride = m->kvd;
+    a.nq = m->nq;
+    a.rows = rows;
+    a.scale = 1.0f / sqrtf((float)m->hd);
+    return a;
+}
+
 int enqueue_decode_step(tmg_model *m, tmg_cache *c, LaunchRecorder *rec, int mode) {
     hipStream_t s = m->stream;
     const int H = m->H, I = m->I, qd = m->qd, kvd = m->kvd;
@@ -424,10 +446,12 @@ int enqueue_decode_step(tmg_model *m, tmg_cache *c, LaunchRecorder *rec, int mod
     const double wb = m->i8 ? 1.0 : 2.0, sb = m->i8 ? 4.0 : 0.0;
     for (int l = 0; l < m->L; l++) {
         const tmg_model::Layer &ly = m->layers[l];
-        float *kc = c->k + (size_t)l * c->max_pos * kvd;
-        float *vc = c->v + (size_t)l * c->max_pos * kvd;
+        // a 4-bit cache's new row goes to the attention as f32
+        float *kc = c->kv4 ? m->kv4_k : c->k + (size_t)l * c->max_pos * kvd;
+        float *vc = c->kv4 ? m->kv4_v : c->v + (size_t)l * c->max_pos * kvd;
 
         GemvArgs qa{};
+        qa.kv_one_row = c->kv4 != nullptr;
         qa.W = ly.qkv;
         qa.out = m->qkv_rows;
         qa.in = H;
@@ -475,7 +499,15 @@ int enqueue_decode_step(tmg_model *m, tmg_cache *c, LaunchRecorder *rec, int mod
         aa.part = m->attn_part;
         aa.part_ml = m->attn_ml;
         aa.out_f32 = c->attn_nsplit == 1 ? m->attn_out : nullptr;
-        if (!rec || rec->want("attn_decode", 2.0 * n_ctx_est * kvd * 4 + 2.0 * qd * 4)) TMG_HIP(launch_attn(aa, s));
+        if (c->kv4) {
+            Kv4AttnArgs ka = kv4_args(m, c, l, m->q, kc, vc, 1);
+            ka.pos_dev = &c->st->pos;
+            ka.out = m->attn_out;
+            if (!rec || rec->want("attn_decode_kv4", n_ctx_est * m->nkv * (m->hd + 2.0 * kv4_groups(m->hd)) + 2.0 * (kvd + qd) * 4))
+                TMG_HIP(launch_kv4_attn(ka, m->kv4_ws, s));
+        } else if (!rec || rec->want("attn_decode", 2.0 * n_ctx_est * kvd * 4 + 2.0 * qd * 4)) {
+            TMG_HIP(launch_attn(aa, s));
+        }
         const bool fused = fused_merge(m, c);
         if (c->attn_nsplit > 1 && !fused) {
             aa.out_f32 = m->attn_out;
@@ -690,11 +722,37 @@ static int ensure_kv_split(tmg_model *m, int n) {
     return TMG_OK;
 }
 
+// The attention's workspace and the rows of decode steps, for 4-bit caches.
+static int ensure_kv4(tmg_model *m) {
+    if (m->kv4_ws) return TMG_OK;
+    int rc;
+    char *ws = nullptr;
+    const size_t bytes = kv4_attn_most_ws_bytes(m->hd);
+    if ((!m->kv4_k && (rc = dev_alloc(m, &m->kv4_k, (size_t)m->kvd))) ||
+        (!m->kv4_v && (rc = dev_alloc(m, &m->kv4_v, (size_t)m->kvd))) || (rc = dev_alloc(m, &ws, bytes)))
+        return rc;
+    if (hipMemset(ws, 0, bytes) != hipSuccess || hipDeviceSynchronize() != hipSuccess)
+        return set_error(TMG_E_DEVICE, "hipMemset failed");
+    m->kv4_ws = ws;
+    return TMG_OK;
+}
+
+// A prefill's f32 key and value rows on their way into a 4-bit cache.
+static int ensure_kv4_rows(tmg_model *m, int T) {
+    if (T <= m->kv4_cap) return TMG_OK;
+    int rc;
+    const int cap = std::max(T, 64);
+    if ((rc = dev_alloc(m, &m->kv4_pk, (size_t)cap * m->kvd)) || (rc = dev_alloc(m, &m->kv4_pv, (size_t)cap * m->kvd)))
+        return rc;
+    m->kv4_cap = cap;
+    return TMG_OK;
+}
+
 // The layers of a batched prefill over T token rows, from m->pf_tokens to the
-// residual rows m->pf_x: one sequence at positions start .. in the cache k / v,
+// residual rows m->pf_x: one sequence at positions start .. in the cache c,
 // or with `rows` several, row n at position rows->pos[n] of the sequence whose
 // caches are rows->k[n] / rows->v[n].
-static int prefill_layers(tmg_model *m, int T, int start, float *k, float *v, uint32_t max_pos,
+static int prefill_layers(tmg_model *m, int T, int start, const tmg_cache *c, uint32_t max_pos,
                           const PrefillRows *rows) {
     const int H = m->H, I = m->I, qd = m->qd, kvd = m->kvd;
     hipStream_t s = m->stream;
@@ -728,8 +786,9 @@ static int prefill_layers(tmg_model *m, int T, int start, float *k, float *v, ui
     for (int l = 0; l < m->L; l++) {
         const tmg_model::Layer &ly = m->layers[l];
         const size_t layer_off = (size_t)l * max_pos * kvd;
-        float *kc = rows ? nullptr : k + layer_off;
-        float *vc = rows ? nullptr : v + layer_off;
+        const bool kv4 = c && c->kv4;
+        float *kc = rows ? nullptr : kv4 ? m->kv4_pk : c->k + layer_off;
+        float *vc = rows ? nullptr : kv4 ? m->kv4_pv : c->v + layer_off;
         const bool in_handed = hand_off && l > 0;
         if (!in_handed) TMG_HIP(launch_rmsnorm_split(m->pf_x, ly.in_norm, eps, T, H, m->pf_hi, m->pf_lo, s));
         GemmArgs g{};
@@ -749,6 +808,7 @@ static int prefill_layers(tmg_model *m, int T, int start, float *k, float *v, ui
         g.q_out = m->pf_q;
         g.k_cache = kc;
         g.v_cache = vc;
+        if (kv4) g.kv_row0 = start;
         if (rows) {
             g.pos_seq = rows->pos;
             g.k_seq = rows->k;
@@ -784,7 +844,13 @@ static int prefill_layers(tmg_model *m, int T, int start, float *k, float *v, ui
                       "attention runs fit the workspace");
         aa.part = m->pf_part;
         aa.part_ml = m->pf_part + (size_t)kAttnRuns * 128 * 128;
-        if (rows) {
+        if (kv4) {
+            Kv4AttnArgs ka = kv4_args(m, c, l, m->pf_q, kc, vc, T);
+            ka.pos = start;
+            ka.out_hi = m->pf_ahi;
+            ka.out_lo = m->pf_alo;
+            TMG_HIP(launch_kv4_attn(ka, m->kv4_ws, s));
+        } else if (rows) {
             aa.pos_seq = rows->pos;
             aa.k_seq = rows->k;
             aa.v_seq = rows->v;
@@ -889,7 +955,7 @@ static int stage_tokens(tmg_model *m, const uint32_t *tokens, size_t T) {
 int run_prefill_rows(tmg_model *m, const uint32_t *tokens, size_t n, uint32_t max_pos, const PrefillRows &rows) {
     int rc;
     if ((rc = stage_tokens(m, tokens, n))) return rc;
-    return prefill_layers(m, (int)n, 0, nullptr, nullptr, max_pos, &rows);
+    return prefill_layers(m, (int)n, 0, nullptr, max_pos, &rows);
 }
 
 int run_prefill_head(tmg_model *m, int row) { return prefill_head(m, row); }
@@ -903,7 +969,8 @@ int run_prefill(tmg_model *m, tmg_cache *c, const uint32_t *tokens, size_t n) {
     if ((rc = ensure_prefill(m, T))) return rc;
     if ((rc = ensure_rope(m, (int)c->len + T + 1))) return rc;
     if ((rc = stage_tokens(m, tokens, n))) return rc;
-    if ((rc = prefill_layers(m, T, (int)c->len, c->k, c->v, c->max_pos, nullptr))) return rc;
+    if (c->kv4 && (rc = ensure_kv4_rows(m, T))) return rc;
+    if ((rc = prefill_layers(m, T, (int)c->len, c, c->max_pos, nullptr))) return rc;
     if ((rc = prefill_head(m, T - 1))) return rc;
     c->len += (uint32_t)T;
     // the device position follows the host mirror after a prefill
@@ -980,9 +1047,17 @@ extern "C" int tmg_model_config(const tmg_model *m, tmg_config *out) {
     return TMG_OK;
 }
 
-extern "C" int tmg_cache_new(tmg_model *m, uint32_t max_pos, tmg_cache **out) {
+extern "C" int tmg_cache_new(tmg_model *m, uint32_t max_pos, tmg_cache **out) { return cache_new(m, max_pos, false, out); }
+
+extern "C" int tmg_cache_new_kv4(tmg_model *m, uint32_t max_pos, tmg_cache **out) {
+    return cache_new(m, max_pos, true, out);
+}
+
+int tmg::cache_new(tmg_model *m, uint32_t max_pos, bool kv4, tmg_cache **out) {
     clear_error();
     if (!m || !out || max_pos == 0) return set_error(TMG_E_INVALID, "bad argument to tmg_cache_new");
+    if (kv4 && !tmg_kv4_bytes(max_pos, (uint32_t)m->nkv, (uint32_t)m->hd))
+        return set_error(TMG_E_INVALID, "no 4-bit cache of this size for the model's heads");
     *out = nullptr;
     (void)hipSetDevice(m->device);
     {
@@ -996,7 +1071,9 @@ extern "C" int tmg_cache_new(tmg_model *m, uint32_t max_pos, tmg_cache **out) {
     // Short caches deal the context to at most kFusedSplits splits in small
     // blocks: at 64-320 positions (1B) 5-8 workgroups per KV head of 16-40
     // positions each instead of 2-5 of 64, the merge still fused into o_proj.
-    if (max_pos <= (uint32_t)kShortAttnCache) {
+    if (kv4) {
+        c->attn_nsplit = 1;  // the 4-bit attention splits and merges by itself
+    } else if (max_pos <= (uint32_t)kShortAttnCache) {
         c->attn_block = attn_chunk(m->hd, m->nq / m->nkv, kAttnThreads, kAttnBlockShort);
         c->attn_nsplit = (int)std::min<uint32_t>(kFusedSplits, (max_pos + c->attn_block - 1) / c->attn_block);
     } else {
@@ -1005,13 +1082,17 @@ extern "C" int tmg_cache_new(tmg_model *m, uint32_t max_pos, tmg_cache **out) {
     }
     const size_t n = (size_t)m->L * max_pos * m->kvd;
     int rc = TMG_OK;
-    void *k = nullptr, *v = nullptr, *st = nullptr, *hist = nullptr;
-    if (hipMalloc(&k, n * 4) != hipSuccess || hipMalloc(&v, n * 4) != hipSuccess ||
+    void *k = nullptr, *v = nullptr, *q4 = nullptr, *st = nullptr, *hist = nullptr;
+    const size_t bytes = kv4 ? (size_t)m->L * kv4_slab_bytes(max_pos, m->nkv, m->hd) : 2 * n * 4;
+    if (kv4) rc = ensure_kv4(m);
+    if (!rc && ((kv4 ? hipMalloc(&q4, bytes) != hipSuccess
+                     : hipMalloc(&k, n * 4) != hipSuccess || hipMalloc(&v, n * 4) != hipSuccess) ||
         hipMalloc(&st, sizeof(DevState)) != hipSuccess ||
-        hipHostMalloc(&hist, ((size_t)max_pos + 2) * 4, hipHostMallocCoherent | hipHostMallocMapped) != hipSuccess)
-        rc = set_error(TMG_E_NOMEM, "KV cache allocation of " + std::to_string(2 * n * 4) + " bytes failed");
+        hipHostMalloc(&hist, ((size_t)max_pos + 2) * 4, hipHostMallocCoherent | hipHostMallocMapped) != hipSuccess))
+        rc = set_error(TMG_E_NOMEM, "KV cache allocation of " + std::to_string(bytes) + " bytes failed");
     c->k = (float *)k;
     c->v = (float *)v;
+    c->kv4 = (uint8_t *)q4;
     c->st = (DevState *)st;
     c->history = (int *)hist;
     const size_t seen_words = ((size_t)m->V + 31) / 32;
@@ -1065,6 +1146,7 @@ extern "C" void tmg_cache_free(tmg_cache *c) {
     (void)hipFree(c->draws);
     (void)hipFree(c->k);
     (void)hipFree(c->v);
+    (void)hipFree(c->kv4);
     (void)hipFree(c->st);
     (void)hipHostFree(c->history);
     tmg_model *m = c->model;
@@ -1101,6 +1183,25 @@ extern "C" int tmg_cache_read(const tmg_cache *c, uint32_t layer, float *keys, f
     (void)hipSetDevice(m->device);
     TMG_HIP(hipStreamSynchronize(m->stream));
     const size_t off = (size_t)layer * c->max_pos * m->kvd, bytes = (size_t)c->len * m->kvd * 4;
+    if (c->kv4) {
+        // through a device buffer of f32 rows
+        if (!bytes || (!keys && !values)) return TMG_OK;
+        void *rows = nullptr;
+        if (hipMalloc(&rows, bytes) != hipSuccess) return set_error(TMG_E_NOMEM, "allocation of the f32 rows failed");
+        hipError_t e = hipSuccess;
+        for (int i = 0; i < 2 && e == hipSuccess; i++) {
+            float *const dst = i ? values : keys;
+            if (!dst) continue;
+            Kv4ReadArgs a{kv4_layer(c, (int)layer), i ? nullptr : (float *)rows, i ? (float *)rows : nullptr, (size_t)m->kvd,
+                          (int)c->len, nullptr, 0};
+            e = launch_kv4_read(a, m->stream);
+            if (e == hipSuccess) e = hipMemcpyAsync(dst, rows, bytes, hipMemcpyDeviceToHost, m->stream);
+            if (e == hipSuccess) e = hipStreamSynchronize(m->stream);
+        }
+        (void)hipFree(rows);
+        TMG_HIP(e);
+        return TMG_OK;
+    }
     if (keys && bytes) TMG_HIP(hipMemcpy(keys, c->k + off, bytes, hipMemcpyDeviceToHost));
     if (values && bytes) TMG_HIP(hipMemcpy(values, c->v + off, bytes, hipMemcpyDeviceToHost));
     return TMG_OK;

@@ -69,6 +69,13 @@ struct tmg_model {
     uint16_t *pf_kh = nullptr, *pf_kl = nullptr, *pf_vth = nullptr, *pf_vtl = nullptr;
     uint8_t *pf_vodd = nullptr;  // per 64-key block and KV head: infinite or NaN values
 
+    // 4-bit caches: the attention's workspace, the f32 key and value row of a
+    // decode step, and a prefill's rows [kv4_cap][kvd] each
+    void *kv4_ws = nullptr;
+    float *kv4_k = nullptr, *kv4_v = nullptr;
+    float *kv4_pk = nullptr, *kv4_pv = nullptr;
+    int kv4_cap = 0;
+
     // pinned host staging
     void *pin = nullptr;
     size_t pin_bytes = 0;
@@ -89,6 +96,7 @@ struct tmg_cache {
     tmg_model *model = nullptr;
     uint32_t max_pos = 0;
     float *k = nullptr, *v = nullptr;  // [L][max_pos][kvd]
+    uint8_t *kv4 = nullptr;            // 4-bit cache instead: a slab of kv4_slab_bytes per layer
     tmg::DevState *st = nullptr;       // device
     // generated ids, max_pos + 2 entries, in coherent pinned host memory that
     // the kernels write directly (the host reads a token as soon as the step
@@ -154,6 +162,10 @@ enum SelectMode {
     SEL_FULL = 3,            // temperature sampling, any other top_k / top_p
 };
 
+// The 4-bit slab of a layer, as the kernels take it.
+Kv4Cache kv4_layer(const tmg_cache *c, int layer);
+// tmg_cache_new, or with kv4 tmg_cache_new_kv4.
+int cache_new(tmg_model *m, uint32_t max_pos, bool kv4, tmg_cache **out);
 int enqueue_decode_step(tmg_model *m, tmg_cache *c, LaunchRecorder *rec, int mode);
 int enqueue_select(tmg_model *m, tmg_cache *c, int mode, int advance_pos);
 // The attention form of a step writing position pos (1: every split active

@@ -248,12 +248,13 @@ struct Kv4Values {
 
     // Whether some group of this lane's keys is marked as not finite; its
     // values are then taken as finite ones (a masked key's weight of zero
-    // must not meet a NaN), and nan_values puts the NaN where it belongs.
+    // must not meet a NaN), and nan_values puts the NaN where it belongs.  So
+    // do the scales past the largest, which only rows never written can hold.
     __device__ __forceinline__ bool take_bad(uint32_t *bits) {
         uint32_t b = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            if (scale[j] == kKv4BadScale) {
+            if (scale[j] > kKv4MaxScale) {
                 b |= 1u << j;
                 scale[j] = 127;
             }
@@ -853,7 +854,7 @@ struct Kv4Stage {
         uint32_t bad = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            if (scale[j] == kKv4BadScale) {
+            if (scale[j] > kKv4MaxScale) {
                 bad |= 1u << j;
                 scale[j] = 127;
             }

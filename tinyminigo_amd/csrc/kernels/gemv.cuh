@@ -292,12 +292,12 @@ __device__ __forceinline__ void gemv_epilogue(const GemvArgs &a, int blk, int po
                             a.q_out[head * a.hd + j] = oa;
                             a.q_out[head * a.hd + j + half] = ob;
                         } else {
-                            float *kr = a.k_cache + (size_t)pos * kvd + (head - a.nq) * a.hd;
+                            float *kr = a.k_cache + (a.kv_one_row ? 0 : (size_t)pos * kvd) + (head - a.nq) * a.hd;
                             kr[j] = oa;
                             kr[j + half] = ob;
                         }
                     } else {
-                        float *vr = a.v_cache + (size_t)pos * kvd + (head - a.nq - a.nkv) * a.hd;
+                        float *vr = a.v_cache + (a.kv_one_row ? 0 : (size_t)pos * kvd) + (head - a.nq - a.nkv) * a.hd;
                         vr[j] = va;
                         vr[j + half] = vb;
                     }

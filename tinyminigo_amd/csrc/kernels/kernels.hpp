@@ -58,6 +58,7 @@ struct GemvArgs {
     int hd, nq, nkv;
     float *q_out;            // [nq*hd]
     float *k_cache, *v_cache;  // layer base, [pos][nkv*hd]
+    int kv_one_row;            // they are one row, written whatever the position (4-bit caches)
     // EPI_LOGITS: one packed (value, row) argmax key per workgroup, or null
     unsigned long long *argmax_part;
     // PRO_ATTN_COMBINE: the activation is the attention output, merged from
@@ -256,6 +257,7 @@ struct GemmArgs {
     int hd, nq, nkv;
     float *q_out;  // [N][nq*hd]
     float *k_cache, *v_cache;
+    int kv_row0;  // the position of their row 0
     // several sequences at once (batched decode): token n is sequence n at
     // position pos_seq[n], its K/V rows go to k_seq[n] / v_seq[n] +
     // kv_layer_off; null pos_seq: one sequence, token n at start + n
@@ -438,6 +440,8 @@ struct Kv4Plan {
     bool split;     // rows kernel: an item may be shared by several workgroups
 };
 Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq);
+// Workspace bytes that no call of this head dim exceeds.
+constexpr size_t kv4_attn_most_ws_bytes(int hd) { return kKv4CounterBytes + (size_t)2 * kKv4Workgroups * 16 * (hd + 2) * 4; }
 // Workspace enough for every position: counters, which are zero between
 // launches, then the partial states.
 size_t kv4_attn_ws_bytes(const Kv4Cache &c, int rows, int nq);

@@ -22,7 +22,7 @@ namespace tmg {
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kKv4BadScale = 255;
+constexpr uint32_t kKv4BadScale = 255, kKv4MaxScale = 252;
 
 // One sequence's planes: a row is (kv head, position).
 template <int HD>
@@ -52,8 +52,8 @@ __device__ __forceinline__ uint32_t kv4_scale_byte(uint32_t bits) {
     return bits >= 0x7F800000u ? kKv4BadScale : (uint32_t)min(max(e, 27), 252);
 }
 
-// The f32 scale of a byte; 255 (f32 infinity's exponent) makes the
-// conversions give NaN.
+// The f32 scale of a byte; infinity, for a marked group, makes the conversions
+// give NaN.
 __device__ __forceinline__ float kv4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // Eight consecutive dimensions of a row, of which LANES consecutive lanes

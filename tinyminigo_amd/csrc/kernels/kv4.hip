@@ -53,7 +53,8 @@ __global__ __launch_bounds__(kBlock) void kv4_read_kernel(const Kv4ReadArgs a) {
         const Kv4Planes<HD> pl(a.c, seq);
         const size_t row = (size_t)g * a.c.cap + p + t;
         const uint32_t c = *reinterpret_cast<const uint32_t *>((val ? pl.vc : pl.kc) + row * (HD / 2) + lane * 4);
-        const float s = kv4_scale((val ? pl.vs : pl.ks)[row * NG + lane / LPG]);
+        const uint32_t b = (val ? pl.vs : pl.ks)[row * NG + lane / LPG];
+        const float s = kv4_scale(b > kKv4MaxScale ? kKv4BadScale : b);
         const f32x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0);
         const f32x2 v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
         const f32x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);

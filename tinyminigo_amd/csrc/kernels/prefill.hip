@@ -140,12 +140,12 @@ __device__ __forceinline__ void gemm_store(const GemmArgs &a, int mb, int n, con
                         qr[j] = oa;
                         qr[j + half] = ob;
                     } else {
-                        float *kr = kcache + (size_t)pos * kvd + (head - a.nq) * a.hd;
+                        float *kr = kcache + (size_t)(pos - a.kv_row0) * kvd + (head - a.nq) * a.hd;
                         kr[j] = oa;
                         kr[j + half] = ob;
                     }
                 } else {
-                    float *vr = vcache + (size_t)pos * kvd + (head - a.nq - a.nkv) * a.hd;
+                    float *vr = vcache + (size_t)(pos - a.kv_row0) * kvd + (head - a.nq - a.nkv) * a.hd;
                     vr[j] = va;
                     vr[j + half] = vb;
                 }
@@ -237,13 +237,13 @@ __device__ __forceinline__ float epi4_finish(const GemmArgs &a, int mb, int n, c
                 dst = a.q_out + (size_t)n * a.nq * a.hd + head * a.hd;
             } else {
                 float *const kcache = a.k_seq ? a.k_seq[n] + a.kv_layer_off : a.k_cache;
-                dst = kcache + (size_t)t.pos * kvd + (head - a.nq) * a.hd;
+                dst = kcache + (size_t)(t.pos - a.kv_row0) * kvd + (head - a.nq) * a.hd;
             }
         } else {
             o0 = make_float2(v[0], v[2]);
             o1 = make_float2(v[1], v[3]);
             float *const vcache = a.v_seq ? a.v_seq[n] + a.kv_layer_off : a.v_cache;
-            dst = vcache + (size_t)t.pos * kvd + (head - a.nq - a.nkv) * a.hd;
+            dst = vcache + (size_t)(t.pos - a.kv_row0) * kvd + (head - a.nq - a.nkv) * a.hd;
         }
         *reinterpret_cast<float2 *>(dst + j) = o0;
         *reinterpret_cast<float2 *>(dst + j + half) = o1;

@@ -115,8 +115,8 @@ class Model:
         except Exception:
             pass
 
-    def new_cache(self, max_pos: int) -> "KvCache":
-        return KvCache(self, max_pos)
+    def new_cache(self, max_pos: int, kv4: bool = False) -> "KvCache":
+        return KvCache(self, max_pos, kv4)
 
     def forward_token(self, token: int, cache: "KvCache", want_logits: bool = True) -> Optional[np.ndarray]:
         """Model::forward_token (src/model.rs:392-491)."""
@@ -175,14 +175,17 @@ class Model:
 
 
 class KvCache:
-    """KvCache (src/model.rs:250-332) as a preallocated HBM slab of max_pos rows."""
+    """KvCache (src/model.rs:250-332) as a preallocated HBM slab of max_pos rows,
+    f32 or with kv4 in 4 bits (tmg_cache_new_kv4)."""
 
-    def __init__(self, model: Model, max_pos: int):
+    def __init__(self, model: Model, max_pos: int, kv4: bool = False):
         self.model = model
         self.max_pos = max_pos
+        self.kv4 = kv4
         self._h = None
         h = C.c_void_p()
-        check(lib.tmg_cache_new(model._h, int(max_pos), C.byref(h)))
+        new = lib.tmg_cache_new_kv4 if kv4 else lib.tmg_cache_new
+        check(new(model._h, int(max_pos), C.byref(h)))
         self._h = h
         model._caches.add(self)
         register(self, 1)
@@ -249,8 +252,9 @@ class GenOutput:
 
 
 def generate(model: Model, prompt_tokens: Sequence[int], params: GenParams,
-             on_token: Optional[Callable[[int], None]] = None) -> GenOutput:
-    """generate (src/model.rs:614-663)."""
+             on_token: Optional[Callable[[int], None]] = None, kv4: bool = False) -> GenOutput:
+    """generate (src/model.rs:614-663), with kv4 over a 4-bit cache
+    (tmg_generate_kv4)."""
     t = _u32(prompt_tokens)
     p = tmg_gen_params(params.max_tokens, params.temperature, params.top_k, params.top_p,
                        params.repetition_penalty, params.seed)
@@ -268,9 +272,9 @@ def generate(model: Model, prompt_tokens: Sequence[int], params: GenParams,
                 err.append(e)
 
     cb = ON_TOKEN(_cb)
-    check(lib.tmg_generate(model._h, t.ctypes.data_as(C.POINTER(C.c_uint32)), t.size, C.byref(p), cb, None,
-                           out.ctypes.data_as(C.POINTER(C.c_uint32)), out.size, C.byref(n_out), _fptr(first),
-                           C.byref(secs)))
+    run = lib.tmg_generate_kv4 if kv4 else lib.tmg_generate
+    check(run(model._h, t.ctypes.data_as(C.POINTER(C.c_uint32)), t.size, C.byref(p), cb, None,
+              out.ctypes.data_as(C.POINTER(C.c_uint32)), out.size, C.byref(n_out), _fptr(first), C.byref(secs)))
     if err:
         raise err[0]
     return GenOutput(tokens=[int(x) for x in out[:n_out.value]], logits_first_step=first,

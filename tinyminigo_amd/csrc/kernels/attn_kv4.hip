@@ -27,7 +27,11 @@
 // dimensions of its eight keys.
 //
 // A column is a (query row, query head) pair of one KV head: column c of a
-// sequence is row c / group, head c % group.
+// sequence is row c / group, head c % group.  Decode steps have two or four
+// columns, not the 16 of a matrix instruction; its other columns then take the
+// parts of the same ones, side by side (Kv4Lanes): one instruction does the
+// scores of 16 keys for two columns instead of six, and one the values'
+// instead of three.
 #include <algorithm>
 
 #include "coh.cuh"
@@ -43,7 +47,7 @@ typedef float f32x32 __attribute__((ext_vector_type(32)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kQParts = 6;
+constexpr int kQParts = 6, kPParts = 3;  // of a query and of a weight
 
 // A barrier for LDS alone: loads from memory stay in flight.
 __device__ __forceinline__ void lds_barrier() {
@@ -52,16 +56,39 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// A column's query in a lane: 128-dimension halves, parts, scale bytes.
-template <int HD>
+// The 16 columns of a matrix operand as C columns of 16 / C parts each: lane r
+// has column r / PARTS of part r % PARTS; what does not fit goes into further
+// sets.  Sums over a column's parts are then sums over PARTS neighbouring
+// lanes.
+template <int C>
+struct Kv4Lanes {
+    static constexpr int PARTS = 16 / C;
+    static constexpr int QSETS = (kQParts + PARTS - 1) / PARTS, PSETS = (kPParts + PARTS - 1) / PARTS;
+    // Every lane gets the sum of its column's parts, and the same bits: a
+    // butterfly adds the same pairs in both of their lanes.  (The half mirror
+    // is the other quad's lane here, all of whose lanes hold its sum.)
+    static __device__ __forceinline__ float sum(float v) {
+        static_assert(PARTS == 1 || PARTS == 4 || PARTS == 8, "one, four or eight lanes a column");
+        if constexpr (PARTS >= 4) v += dpp_mov<kDppXor1>(v);
+        if constexpr (PARTS >= 4) v += dpp_mov<kDppXor2>(v);
+        if constexpr (PARTS >= 8) v += dpp_mov<kDppHalfMirror>(v);
+        return v;
+    }
+};
+
+// A column's query in a lane: 128-dimension halves, sets of parts, scale
+// bytes.
+template <int HD, int C>
 struct Kv4Query {
-    static constexpr int KH = (HD + 127) / 128;
+    static constexpr int KH = (HD + 127) / 128, SETS = Kv4Lanes<C>::QSETS, PARTS = Kv4Lanes<C>::PARTS;
     f32x16 ev[KH], od[KH];  // the lane's even and odd dimensions, until split
-    u32x6 part[KH][kQParts];
-    uint32_t scale[KH][2];  // part n's byte: byte n & 3 of word n >> 2
+    int first[KH];          // the first part's scale byte, 255 for what is not finite
+    float mul[KH];          // what ev and od are still to be scaled by
+    u32x6 part[KH][SETS];
+    uint32_t scale[KH][(SETS + 3) / 4];  // set s's byte: byte s & 3 of word s >> 2
 
     // src: the column's HD floats.  Lanes past the head's dimensions repeat
-    // the first ones; split() takes them as zeros.  (No branch: a loaded value
+    // the first ones; ready() takes them as zeros.  (No branch: a loaded value
     // that meets a constant is waited for on the spot.)
     __device__ __forceinline__ void fetch(const float *src, int lg) {
 #pragma unroll
@@ -82,58 +109,53 @@ struct Kv4Query {
         }
     }
 
-    // Scales by f, for digit().
+    // The first parts' scales of what was fetched, times f.
     __device__ __forceinline__ void ready(float f, int lg) {
 #pragma unroll
         for (int h = 0; h < KH; h++) {
             // (a NaN or an infinity times the zero marks a column that is NaN anyway)
-            const float mul = 128 * h + 32 * lg < HD ? f : 0.f;
-            uint32_t m = 0;
+            mul[h] = 128 * h + 32 * lg < HD ? f : 0.f;
+            float m = 0.f;  // NaN where one is
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                ev[h][i] *= mul;
-                od[h][i] *= mul;
-                m = max(m, max(__float_as_uint(ev[h][i]) & 0x7FFFFFFFu, __float_as_uint(od[h][i]) & 0x7FFFFFFFu));
+            for (int i = 0; i < 16; i++)
+                m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(m, fabsf(ev[h][i])), fabsf(od[h][i]));
+            const uint32_t bits = __float_as_uint(m * fabsf(mul[h]));
+            // the largest magnitude is at most 15/8 of the first part's scale;
+            // 2^126 and more count as infinite
+            first[h] = bits >= 0x7E800000u ? 255 : max((int)(bits >> 23) + ((bits & 0x7FFFFFu) > 0x700000u), 27);
+        }
+    }
+    __device__ __forceinline__ void scales(int pr) {
+#pragma unroll
+        for (int h = 0; h < KH; h++) {
+#pragma unroll
+            for (int w = 0; w < (SETS + 3) / 4; w++) scale[h][w] = 0;
+#pragma unroll
+            for (int set = 0; set < SETS; set++) {
+                const int n = set * PARTS + pr;
+                const int byte = first[h] == 255 || n >= kQParts ? first[h] : first[h] - 4 * n;
+                scale[h][set >> 2] |= (uint32_t)byte << (8 * (set & 3));
             }
-            // the largest magnitude is at most 15/8 of the first part's scale
-            const int e = min(max((int)(m >> 23) + ((m & 0x7FFFFFu) > 0x700000u), 27), 254);
-            const bool bad = m >= 0x7F800000u;
-            scale[h][0] = bad ? 0xFFFFFFFFu : (uint32_t)(e | (e - 4) << 8 | (e - 8) << 16 | (e - 12) << 24);
-            scale[h][1] = bad ? 0xFFFFFFFFu : (uint32_t)((e - 16) | (e - 20) << 8);
         }
     }
 
-    // Part n of half h: with T_n the nearest integer to 8 16^n q / s, the
-    // digit T_n - 16 T_(n - 1).  Any part by itself, so that the wavefronts of
-    // a workgroup can make one each: a conversion takes some 125 clocks.
+    // Part n of half h (zeros past the last): with x = q / (2 s) in units of
+    // 16^-n, what the nearest integer to it leaves, to the nearest sixteenth
+    // (the conversion's rounding); for the first part x itself.  So any part is
+    // made by itself, and lanes or wavefronts make one each: a conversion
+    // takes some 125 clocks.
     __device__ __forceinline__ u32x6 digit(int h, int n) const {
-        const int e = (int)(scale[h][0] & 255);
-        const float f = __uint_as_float((uint32_t)(257 - e + 4 * n) << 23);
-        const float before = n ? __uint_as_float((uint32_t)(253 - e + 4 * n) << 23) : 0.f;
+        // x * mul is rounded as if alone: the rest is a power of two
+        const float g = n < kQParts ? mul[h] * __uint_as_float((uint32_t)(253 - first[h] + 4 * n) << 23) : 0.f;
+        const float whole = n == 0 ? 0.f : -1.f;
         f32x16 a, b;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            a[i] = fmaf(-16.f, rintf(ev[h][i] * before), rintf(ev[h][i] * f));
-            b[i] = fmaf(-16.f, rintf(od[h][i] * before), rintf(od[h][i] * f));
+            const float x = ev[h][i] * g, y = od[h][i] * g;
+            a[i] = fmaf(whole, rintf(x), x);
+            b[i] = fmaf(whole, rintf(y), y);
         }
-        return __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 8.0f);
-    }
-
-    // The parts of half h one after the other: n = 0, 1, ..  What they leave
-    // stays in ev and od.
-    __device__ __forceinline__ u32x6 next_digit(int h, int n) {
-        const int e = (int)(scale[h][0] & 255);
-        const float f = __uint_as_float((uint32_t)(257 - e + 4 * n) << 23);
-        const float back = -__uint_as_float((uint32_t)(e - 3 - 4 * n) << 23);
-        f32x16 a, b;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            a[i] = rintf(ev[h][i] * f);
-            b[i] = rintf(od[h][i] * f);
-            ev[h][i] = fmaf(a[i], back, ev[h][i]);
-            od[h][i] = fmaf(b[i], back, od[h][i]);
-        }
-        return __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 8.0f);
+        return __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(a, b, 0.5f);
     }
 };
 
@@ -146,7 +168,7 @@ struct Kv4SharedQuery {
 #pragma unroll
         for (int i = 0; i < 3; i++) w[h][n][i][lg][r] = make_uint2(p[2 * i], p[2 * i + 1]);
     }
-    __device__ __forceinline__ void get(Kv4Query<HD> &q, int r, int lg) const {
+    __device__ __forceinline__ void get(Kv4Query<HD, 16> &q, int r, int lg) const {
 #pragma unroll
         for (int h = 0; h < KH; h++)
 #pragma unroll
@@ -183,36 +205,43 @@ struct Kv4Key {
     }
 };
 
-// Part N's products of TILES tiles of 16 keys with 16 columns.
-template <int N, int HD, int TILES>
-__device__ __forceinline__ void score_part(const Kv4Key<HD> (&k)[TILES], const Kv4Query<HD> &q, int h, f32x4 (&s)[TILES]) {
-    const u32x6 p = q.part[h][N];
+// Set S's products of TILES tiles of 16 keys with the columns.
+template <int S, int HD, int C, int TILES>
+__device__ __forceinline__ void score_set(const Kv4Key<HD> (&k)[TILES], const Kv4Query<HD, C> &q, int h, f32x4 (&s)[TILES]) {
+    const u32x6 p = q.part[h][S];
     const i32x8 b = {(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)p[4], (int)p[5], 0, 0};
 #pragma unroll
     for (int i = 0; i < TILES; i++) {
         const u32x4 c = k[i].code[h];
         const i32x8 a = {(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0};
         s[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, s[i], 4 /* fp4 */, 2 /* fp6 e2m3 */, 0,
-                                                                (int)k[i].scale[h], N & 3, (int)q.scale[h][N >> 2]);
+                                                                (int)k[i].scale[h], S & 3, (int)q.scale[h][S >> 2]);
+    }
+}
+
+template <int S, int HD, int C, int TILES>
+__device__ __forceinline__ void score_sets(const Kv4Key<HD> (&k)[TILES], const Kv4Query<HD, C> &q, f32x4 (&s)[TILES]) {
+    if constexpr (S < Kv4Lanes<C>::QSETS) {
+#pragma unroll
+        for (int h = 0; h < Kv4Key<HD>::KH; h++) score_set<S>(k, q, h, s);
+        score_sets<S + 1>(k, q, s);
     }
 }
 
 // Scores in log2 units, less `ref`: the sums start from -ref and the largest
 // part, so that what follows is added to numbers as small as the differences.
-template <int HD, int TILES>
-__device__ __forceinline__ void kv4_scores(const Kv4Key<HD> (&k)[TILES], const Kv4Query<HD> &q, float ref, f32x4 (&s)[TILES]) {
+// pr: the lane's part.
+template <int HD, int C, int TILES>
+__device__ __forceinline__ void kv4_scores(const Kv4Key<HD> (&k)[TILES], const Kv4Query<HD, C> &q, float ref, int pr,
+                                           f32x4 (&s)[TILES]) {
+    const float from = pr == 0 ? -ref : 0.f;
 #pragma unroll
-    for (int i = 0; i < TILES; i++) s[i] = f32x4{-ref, -ref, -ref, -ref};
+    for (int i = 0; i < TILES; i++) s[i] = f32x4{from, from, from, from};
+    score_sets<0>(k, q, s);
 #pragma unroll
-    for (int h = 0; h < Kv4Key<HD>::KH; h++) score_part<0>(k, q, h, s);
+    for (int i = 0; i < TILES; i++)
 #pragma unroll
-    for (int h = 0; h < Kv4Key<HD>::KH; h++) {
-        score_part<1>(k, q, h, s);
-        score_part<2>(k, q, h, s);
-        score_part<3>(k, q, h, s);
-        score_part<4>(k, q, h, s);
-        score_part<5>(k, q, h, s);
-    }
+        for (int e = 0; e < 4; e++) s[i][e] = Kv4Lanes<C>::sum(s[i][e]);
 }
 
 // A lane's HD / 16 dimensions of its eight keys of a unit of 32.
@@ -282,34 +311,49 @@ struct Kv4Values {
     }
 };
 
-// Eight weights as three bf16 parts, their upper, middle and lower eight
-// significant bits: exact.
-__device__ __forceinline__ void split_p(const float *p, bf16x8 (&out)[3]) {
-    uint32_t hi[8], mid[8], lo[8];
+// Eight weights as bf16 parts, their upper, middle and lower eight significant
+// bits: exact.  Set by set, the lane's part of each.
+template <int C>
+__device__ __forceinline__ void split_p(const float *p, int pr, bf16x8 (&out)[Kv4Lanes<C>::PSETS]) {
+    static_assert(C == 16 || Kv4Lanes<C>::PSETS == 1, "the parts of a column in one set, or a set each");
+    if constexpr (C == 16) {
+        uint32_t x[kPParts][8];  // the parts are the upper halves
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        hi[j] = __float_as_uint(p[j]) & 0xFFFF0000u;
-        const float m = p[j] - __uint_as_float(hi[j]);
-        mid[j] = __float_as_uint(m);
-        lo[j] = __float_as_uint(m - __uint_as_float(mid[j] & 0xFFFF0000u));
-    }
-    u32x4 a, b, c;
+        for (int j = 0; j < 8; j++) {
+            const float m = p[j] - __uint_as_float(__float_as_uint(p[j]) & 0xFFFF0000u);
+            x[0][j] = __float_as_uint(p[j]);
+            x[1][j] = __float_as_uint(m);
+            x[2][j] = __float_as_uint(m - __uint_as_float(__float_as_uint(m) & 0xFFFF0000u));
+        }
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        // the upper halves of two words
-        a[j] = __builtin_amdgcn_perm(hi[2 * j + 1], hi[2 * j], 0x07060302u);
-        b[j] = __builtin_amdgcn_perm(mid[2 * j + 1], mid[2 * j], 0x07060302u);
-        c[j] = __builtin_amdgcn_perm(lo[2 * j + 1], lo[2 * j], 0x07060302u);
+        for (int n = 0; n < kPParts; n++) {
+            u32x4 a;
+#pragma unroll
+            for (int j = 0; j < 4; j++) a[j] = __builtin_amdgcn_perm(x[n][2 * j + 1], x[n][2 * j], 0x07060302u);
+            out[n] = __builtin_bit_cast(bf16x8, a);
+        }
+    } else {
+        // the lane's part by masks (selects become branches here); lanes past
+        // the last part take zeros by the byte selector
+        const uint32_t m1 = pr >= 1 ? 0xFFFF0000u : 0u, m2 = pr >= 2 ? 0xFFFF0000u : 0u;
+        const uint32_t pick = pr < kPParts ? 0x07060302u : 0x0C0C0C0Cu;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] = p[j] - __uint_as_float(__float_as_uint(p[j]) & m1);
+            x[j] -= __uint_as_float(__float_as_uint(x[j]) & m2);
+        }
+        u32x4 a;
+#pragma unroll
+        for (int j = 0; j < 4; j++) a[j] = __builtin_amdgcn_perm(__float_as_uint(x[2 * j + 1]), __float_as_uint(x[2 * j]), pick);
+        out[0] = __builtin_bit_cast(bf16x8, a);
     }
-    out[0] = __builtin_bit_cast(bf16x8, a);
-    out[1] = __builtin_bit_cast(bf16x8, b);
-    out[2] = __builtin_bit_cast(bf16x8, c);
 }
 
-template <int PARTS>
-__device__ __forceinline__ f32x4 mfma_pv(const u32x4 &v, const bf16x8 (&p)[PARTS], f32x4 o) {
+template <int SETS>
+__device__ __forceinline__ f32x4 mfma_pv(const u32x4 &v, const bf16x8 (&p)[SETS], f32x4 o) {
 #pragma unroll
-    for (int n = PARTS - 1; n >= 0; n--)
+    for (int n = SETS - 1; n >= 0; n--)
         o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), p[n], o, 0, 0, 0);
     return o;
 }
@@ -467,18 +511,23 @@ struct Kv4Item {
     int nb;    // blocks of keys up to it
 };
 
+// p: the sequence's position as given.
 template <int BLOCK>
-__device__ __forceinline__ Kv4Item kv4_item(const Kv4AttnArgs &a, int i) {
+__device__ __forceinline__ Kv4Item kv4_item(const Kv4AttnArgs &a, int i, int p) {
     Kv4Item it;
     it.seq = a.ntile == 1 ? i : i / a.ntile;
     it.tile = i - it.seq * a.ntile;
     it.cols = min(16, a.rows * a.group - 16 * it.tile);
     it.t0 = a.ntile == 1 ? 0 : 16 * it.tile / a.group;
     it.h0 = 16 * it.tile - it.t0 * a.group;
-    it.pos = kv4_pos(a.pos_dev, a.pos, it.seq, a.rows, a.c.cap);
+    it.pos = kv4_pos(p, a.rows, a.c.cap);
     it.last = it.pos + it.t0 + div_group(a, it.h0 + it.cols - 1);
     it.nb = it.pos < 0 ? 0 : it.last / BLOCK + 1;
     return it;
+}
+template <int BLOCK>
+__device__ __forceinline__ Kv4Item kv4_item(const Kv4AttnArgs &a, int i) {
+    return kv4_item<BLOCK>(a, i, a.pos_dev ? a.pos_dev[a.ntile == 1 ? i : i / a.ntile] : a.pos);
 }
 
 // Output element d of the item's column c.
@@ -486,7 +535,7 @@ template <int HD>
 __device__ __forceinline__ void kv4_put(const Kv4AttnArgs &a, const Kv4Item &it, int g, int c, int d, float O, float L) {
     const int dt = div_group(a, it.h0 + c), h = it.h0 + c - dt * a.group;
     const size_t i = ((size_t)it.seq * a.rows + it.t0 + dt) * a.out_stride + (size_t)(g * a.group + h) * HD + d;
-    const float v = L == 0.f ? 0.f : O / L;
+    const float v = L == 0.f ? 0.f : O * __builtin_amdgcn_rcpf(L);  // (the reciprocal is within an ulp)
     if (a.out) a.out[i] = v;
     if (a.out_hi) split_bf16(v, a.out_hi + i, a.out_lo + i);
 }
@@ -522,28 +571,34 @@ constexpr int kv4_waves() {
 //
 // Bound by the latency of its loads and of the merge for one sequence, by the
 // cache's bytes for many.
-template <int HD, bool ONE>
+template <int HD, bool ONE, int C>
 __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) void kv4_attn_rows_kernel(const Kv4AttnArgs a) {
     constexpr int DPL = HD / 16, PITCH = HD + 4, NW = kv4_waves<HD, ONE>(), NT = 64 * NW, BLOCK = 32 * NW;
     // the wavefronts' sums [NW][16][PITCH], then the runs' weights [16][kKv4MaxRuns]
     constexpr int SUMS = NW * 16 * PITCH, WEIGHTS = 16 * kKv4MaxRuns;
     __shared__ __attribute__((aligned(16))) float s_o[SUMS > WEIGHTS ? SUMS : WEIGHTS];
     __shared__ float s_m[16][NW], s_l[16][NW];
-    __shared__ Kv4SharedQuery<HD> s_q;
+    __shared__ Kv4SharedQuery<C == 16 ? HD : 16> s_q;
     __shared__ Kv4NewRow<HD> s_new;
     __shared__ unsigned s_arrived;
     __shared__ int s_first[ONE ? 1 : kKv4FlatItems + 1];  // the items' first blocks in the row of all
     __shared__ int s_sum[NW], s_start;
     __shared__ float s_red[NT];
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r = lane & 15, lg = lane >> 4;
-    const int g = (int)(blockIdx.x % (unsigned)a.c.nkv), run = (int)(blockIdx.x / (unsigned)a.c.nkv);
+    // (run, KV head): one item's runs read different keys; several items' tiles
+    // share a head's, whose workgroups are nkv apart, so on one XCD for eight
+    const int g = ONE ? (int)blockIdx.y : (int)(blockIdx.x % (unsigned)a.c.nkv);
+    const int run = ONE ? (int)blockIdx.x : (int)(blockIdx.x / (unsigned)a.c.nkv);
     const size_t row0 = (size_t)g * a.c.cap;
     const bool append = a.k_new != nullptr;
 
     Kv4Key<HD> k[2];
     Kv4Values<HD> v;
-    Kv4Query<HD> q;
+    Kv4Query<HD, C> q;
     float xn[8];
+    // the lane's column and part
+    constexpr int PARTS = Kv4Lanes<C>::PARTS;
+    const int rc = r / PARTS, pr = r % PARTS;
     // keys key0 .. +31 of the head; those past lim repeat it
     auto load = [&](const Kv4Planes<HD> &pl, int key0, int lim) {
         const int at = min(key0, lim), d = lim - at;
@@ -554,7 +609,7 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
         v.load(pl.vc + row * (HD / 2), pl.vs + row * kv4_groups(HD), d, r, lg);
     };
     auto fetch = [&](int seq, int t0, int h0, int cols) {
-        const int c = h0 + min(r, cols - 1), dt = div_group(a, c), h = c - dt * a.group;
+        const int c = h0 + min(rc, cols - 1), dt = div_group(a, c), h = c - dt * a.group;
         q.fetch(a.q + ((size_t)seq * a.rows + t0 + dt) * a.q_stride + (size_t)(g * a.group + h) * HD, lg);
         if (append) {
             const int l = lane % (HD / 4);
@@ -564,6 +619,29 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
         }
     };
 
+    // the query's parts, from what was fetched
+    auto split = [&](int cols) {
+        q.ready(a.scale * 1.4426950408889634f, lg);
+        q.scales(pr);
+#pragma unroll
+        for (int h = 0; h < Kv4Query<HD, C>::KH; h++) {
+            if constexpr (C < 16) {  // a lane makes its own
+#pragma unroll
+                for (int set = 0; set < Kv4Lanes<C>::QSETS; set++) q.part[h][set] = q.digit(h, set * PARTS + pr);
+            } else {  // the wavefronts make them together
+                for (int n = wave; n < kQParts; n += NW) {
+                    const u32x6 d = q.digit(h, n);
+                    if (r < cols) s_q.put(d, h, n, r, lg);
+                }
+            }
+        }
+        if constexpr (C == 16) {
+            lds_barrier();  // the keys may still be on their way
+            s_q.get(q, min(r, cols - 1), lg);
+        }
+    };
+
+    int pos0 = a.pos;
     int item = 0, x = 0, xend = 1;  // blocks [x, xend) of all the items'
     int per = 1, total = 0;         // blocks of a run, of all items
     const bool flat = !ONE && a.flat;
@@ -572,6 +650,13 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
         fetch(0, 0, 0, min(16, a.rows * a.group));
         load(Kv4Planes<HD>(a.c, 0), run * BLOCK + 32 * wave, (int)a.c.cap - 1);
         asm volatile("" ::: "memory");  // not behind the position's read
+        if (a.pos_dev) pos0 = *a.pos_dev;
+        split(min(16, a.rows * a.group));
+        if constexpr (C < 16)  // made here, while the position is on its way
+#pragma unroll
+            for (int h = 0; h < Kv4Query<HD, C>::KH; h++)
+#pragma unroll
+                for (int set = 0; set < Kv4Lanes<C>::QSETS; set++) asm volatile("" : "+v"(q.part[h][set]));
     } else if (flat) {
         constexpr int PER = (kKv4FlatItems + NT - 1) / NT;
         int n[PER], sum = 0;
@@ -614,7 +699,7 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
     }
     const int x_begin = x;
     for (; x < xend; item++) {
-        const Kv4Item it = kv4_item<BLOCK>(a, item);
+        const Kv4Item it = ONE ? kv4_item<BLOCK>(a, 0, pos0) : kv4_item<BLOCK>(a, item);
         const Kv4Planes<HD> pl(a.c, it.seq);
         // this workgroup's blocks b, b + step, .. < bend of the item, which
         // `parts` workgroups share, the first of them run r0
@@ -646,24 +731,15 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
         Kv4State<HD> st;
         if (pos >= 0) {
             // (lanes past the columns repeat the last one)
-            const int qpos = pos + it.t0 + div_group(a, it.h0 + min(r, cols - 1));
+            const int qpos = pos + it.t0 + div_group(a, it.h0 + min(rc, cols - 1));
             const int first_pos = pos + it.t0;
             int key0 = b * BLOCK + 32 * wave;
             const int end = min(bend * BLOCK, it.last + 1);
             if constexpr (!ONE) {
                 fetch(it.seq, it.t0, it.h0, cols);
                 load(pl, key0, it.last);
+                split(cols);
             }
-            // the wavefronts make the query's parts together
-            q.ready(a.scale * 1.4426950408889634f, lg);
-#pragma unroll
-            for (int h = 0; h < Kv4Query<HD>::KH; h++)
-                for (int n = wave; n < kQParts; n += NW) {
-                    const u32x6 d = q.digit(h, n);
-                    if (r < cols) s_q.put(d, h, n, r, lg);
-                }
-            lds_barrier();  // the keys may still be on their way
-            s_q.get(q, min(r, cols - 1), lg);
             for (; key0 < end; key0 += step * BLOCK) {
                 if (append && key0 + 31 >= pos) {
                     s_new.put(xn, lane, pl, row0 + pos);
@@ -673,7 +749,7 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
                     s_new.patch(k, v, pos - key0, r, lg);
                 }
                 f32x4 s[2];
-                kv4_scores(k, q, st.ref, s);
+                kv4_scores(k, q, st.ref, pr, s);
                 Kv4Values<HD> vn = v;
                 if (key0 + step * BLOCK < end) load(pl, key0 + step * BLOCK, it.last);
                 if (key0 + 31 > first_pos) {
@@ -683,8 +759,8 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
                 }
                 float p[8];
                 st.weights(s, p);
-                bf16x8 pp[3];
-                split_p(p, pp);
+                bf16x8 pp[Kv4Lanes<C>::PSETS];
+                split_p<C>(p, pr, pp);
                 uint32_t bad;
                 const bool any_bad = vn.take_bad(&bad);
                 kv4_values(vn, pp, st.o);
@@ -694,18 +770,19 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
         }
         // the wavefronts' states
         st.l = add_xor32(add_xor16(st.l));
-        if (r < cols) {
+        constexpr int OPARTS = C < 16 ? kPParts : 1;  // lanes with parts of a column's sums
+        if (rc < cols && pr < OPARTS) {
             float *const dst = s_o + (wave * 16 + r) * PITCH + 4 * lg * DPL;
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int d = 0; d < DPL; d++) dst[i * DPL + d] = st.o[d][i];
-            if (lg == 0) {
-                s_m[r][wave] = st.max_ref();
-                s_l[r][wave] = st.l;
+            if (lg == 0 && pr == 0) {
+                s_m[rc][wave] = st.max_ref();
+                s_l[rc][wave] = st.l;
             }
         }
-        __syncthreads();
+        lds_barrier();  // (an appended row's stores may still be on their way)
         // partial states: two slots a run, the second for an item that the
         // run begins after another
         const size_t slot = ((size_t)g * a.runs + run) * 2 + (begun ? 1 : 0);
@@ -721,7 +798,10 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
                 // they are zeros, or NaN
                 const float f = s_m[c][w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[c][w] - M);
                 L = fmaf(s_l[c][w], f, L);
-                O = fmaf(s_o[(w * 16 + c) * PITCH + d], f, O);
+                float sum = s_o[(w * 16 + c * PARTS) * PITCH + d];
+#pragma unroll
+                for (int e = 1; e < OPARTS; e++) sum += s_o[(w * 16 + c * PARTS + e) * PITCH + d];
+                O = fmaf(sum, f, O);
             }
             if (parts == 1) {
                 kv4_put<HD>(a, it, g, c, d, O, L);
@@ -766,6 +846,9 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
                     float M = -INFINITY, L = 0.f, m[FAR], l[FAR];
 #pragma unroll
                     for (int i = 0; i < FAR; i++) {
+                        m[i] = -INFINITY;
+                        l[i] = 0.f;
+                        if (64 * i >= parts) continue;
                         const float *ml = a.part_ml + (part(min(lane + 64 * i, parts - 1)) + c) * 2;
                         m[i] = ld_dev(ml);
                         l[i] = ld_dev(ml + 1);
@@ -775,6 +858,7 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
                     M = wave_max(M);
 #pragma unroll
                     for (int i = 0; i < FAR; i++) {
+                        if (64 * i >= parts) continue;
                         const bool there = lane + 64 * i < parts;
                         const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - M);
                         L = there ? fmaf(l[i], f, L) : L;
@@ -926,7 +1010,7 @@ __global__ __launch_bounds__(kBlock, 2) void kv4_attn_tile_kernel(const Kv4AttnA
     const size_t row0 = (size_t)g * a.c.cap;
 
     int col[CT], qpos[CT];  // in the tile; lanes past the columns repeat the last one
-    Kv4Query<HD> q[CT];
+    Kv4Query<HD, 16> q[CT];
     Kv4State<HD> st[CT];
     const bool mine = 16 * CT * wave < cols;
 #pragma unroll
@@ -962,12 +1046,13 @@ __global__ __launch_bounds__(kBlock, 2) void kv4_attn_tile_kernel(const Kv4AttnA
 #pragma unroll
     for (int c = 0; c < CT; c++) {
         q[c].ready(a.scale * 1.4426950408889634f, lg);
+        q[c].scales(0);
         // through LDS, so that the parts are made in a loop: unrolled they
         // are most of the kernel's code
 #pragma unroll
-        for (int h = 0; h < Kv4Query<HD>::KH; h++)
+        for (int h = 0; h < Kv4Query<HD, 16>::KH; h++)
 #pragma unroll 1
-            for (int n = 0; n < kQParts; n++) s_q[wave].put(q[c].next_digit(h, n), h, n, r, lg);
+            for (int n = 0; n < kQParts; n++) s_q[wave].put(q[c].digit(h, n), h, n, r, lg);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         s_q[wave].get(q[c], r, lg);
@@ -987,7 +1072,7 @@ __global__ __launch_bounds__(kBlock, 2) void kv4_attn_tile_kernel(const Kv4AttnA
         if (work) {
             f32x4 s[CT][4];
 #pragma unroll
-            for (int c = 0; c < CT; c++) kv4_scores(k, q[c], st[c].ref, s[c]);
+            for (int c = 0; c < CT; c++) kv4_scores(k, q[c], st[c].ref, 0, s[c]);
             load_keys(key0 + kTileKeys);
 #pragma unroll
             for (int c = 0; c < CT; c++) {
@@ -998,8 +1083,8 @@ __global__ __launch_bounds__(kBlock, 2) void kv4_attn_tile_kernel(const Kv4AttnA
                 }
                 float w[16];
                 st[c].weights(s[c], w);
-                split_p(w, p[c][0]);
-                split_p(w + 8, p[c][1]);
+                split_p<16>(w, 0, p[c][0]);
+                split_p<16>(w + 8, 0, p[c][1]);
             }
         }
         // the next block's values, while this one's are multiplied
@@ -1087,14 +1172,27 @@ size_t kv4_attn_ws_bytes(const Kv4Cache &c, int rows, int nq) {
 
 namespace {
 
+// Columns of an item in as few lanes as hold them: two or four with their
+// parts beside them, or 16.
+template <int HD, bool ONE>
+void launch_rows(const Kv4AttnArgs &a, unsigned grid, hipStream_t s) {
+    const dim3 block(64 * kv4_waves<HD, ONE>()), wgs = ONE ? dim3(a.runs, a.c.nkv) : dim3(grid);
+    if (a.part_cols <= 2)
+        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, ONE, 2>), wgs, block, 0, s, a);
+    else if (a.part_cols <= 4)
+        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, ONE, 4>), wgs, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, ONE, 16>), wgs, block, 0, s, a);
+}
+
 template <int HD>
 void launch_attn_hd(const Kv4AttnArgs &a, bool tile, unsigned grid, hipStream_t s) {
     if (tile)
         hipLaunchKernelGGL((kv4_attn_tile_kernel<HD>), dim3(grid), dim3(kBlock), 0, s, a);
     else if (a.items == 1)
-        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, true>), dim3(grid), dim3(64 * kv4_waves<HD, true>()), 0, s, a);
+        launch_rows<HD, true>(a, grid, s);
     else
-        hipLaunchKernelGGL((kv4_attn_rows_kernel<HD, false>), dim3(grid), dim3(64 * kv4_waves<HD, false>()), 0, s, a);
+        launch_rows<HD, false>(a, grid, s);
 }
 
 }  // namespace

@@ -41,9 +41,11 @@ struct Kv4Planes {
 
 // A sequence's first row position, or -1 where it takes no part: an idle
 // slot, or rows that would pass the capacity.
-__device__ __forceinline__ int kv4_pos(const int *pos_dev, int pos, int seq, int rows, uint32_t cap) {
-    const int p = pos_dev ? pos_dev[seq] : pos;
+__device__ __forceinline__ int kv4_pos(int p, int rows, uint32_t cap) {
     return p < 0 || (int64_t)p + rows > (int64_t)cap ? -1 : p;
+}
+__device__ __forceinline__ int kv4_pos(const int *pos_dev, int pos, int seq, int rows, uint32_t cap) {
+    return kv4_pos(pos_dev ? pos_dev[seq] : pos, rows, cap);
 }
 
 // Scale byte of a group whose largest |x| has these f32 bits.

@@ -278,19 +278,19 @@ def test_attn_prompts_of_many_sequences(T, H, hd, group, n):
     ones, one column past a tile, idle slots, values and keys that are not
     finite, strided rows."""
     rng = np.random.default_rng(hd + group + n)
-    c = Cache(T, H, n + 150, 4, hd, n_seq=64, gap=32)
+    c = Cache(T, H, n + 150, 4, hd, n_seq=128, gap=32)
 
     def spoil(k, at):
         k[5, at, 1, hd // 2] = np.nan
         k[7, at + 60, 0, 0] = np.inf
         return k
     c.fill(rng, n + 140, keys=lambda k: spoil(k, 61), values=lambda v: spoil(v, 63))
-    pos = [int(x) for x in rng.integers(0, 140, 64)]
+    pos = [int(x) for x in rng.integers(0, 140, 128)]
     pos[0], pos[1], pos[2], pos[3], pos[4], pos[5], pos[7] = 0, 150, -1, 151, 64, 40, 61
-    q = rng.standard_normal((64, n, 4 * group, hd)).astype(np.float32)
+    q = rng.standard_normal((128, n, 4 * group, hd)).astype(np.float32)
     w = 4 * group * hd
     got = attend(c, q, pos, dev=ints(H, pos), q_stride=w + 4, out_stride=w + 12)
-    check_attn(c, got, q, pos, only=(0, 1, 2, 3, 4, 5, 7, 8, 63))
+    check_attn(c, got, q, pos, only=(0, 1, 2, 3, 4, 5, 7, 8, 127))
     # appended first: the same rows as written by themselves
     new = rows(rng, c, n), rows(rng, c, n)
     got = attend(c, q, pos, dev=ints(H, pos), new=new)

@@ -900,11 +900,10 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
 
 // ---- many columns -----------------------------------------------------------
 
-// Column tiles of 16 of a wavefront; a workgroup is four wavefronts.
-template <int HD>
-constexpr int kv4_col_tiles() {
-    return HD == 256 ? 1 : 2;
-}
+// Column tiles of 16 of a wavefront; a workgroup is four wavefronts.  With one,
+// three wavefronts fit a SIMD: 8192 tokens 548 us, against 703 with two tiles
+// and two wavefronts.
+constexpr int kColTiles = 1;
 constexpr int kTileKeys = 64;  // keys of a block
 
 // A wavefront's share of widening a block's values: a unit of 32 keys, and
@@ -979,17 +978,17 @@ struct Kv4Stage {
     }
 };
 
-// Long prompts: a workgroup owns a tile of 64 kv4_col_tiles() columns, 16
-// kv4_col_tiles() a wavefront, and goes through their blocks of 64 keys.  The
+// Long prompts: a workgroup owns a tile of 64 kColTiles columns, 16 kColTiles
+// a wavefront, and goes through their blocks of 64 keys.  The
 // wavefronts read the block's keys straight into matrix operands; the values
 // are widened once for all of them, a share each, into LDS in operand order (a
 // lane's operand is 16 bytes at 16 lane: no bank conflicts), a block ahead.
 //
 // Workgroups of the latest positions come first: they have the most keys.
-// Bound by the MFMA and VALU issue of its two wavefronts a SIMD.
+// Bound by the MFMA and VALU issue of its three wavefronts a SIMD.
 template <int HD>
-__global__ __launch_bounds__(kBlock, 2) void kv4_attn_tile_kernel(const Kv4AttnArgs a) {
-    constexpr int DPL = HD / 16, CT = kv4_col_tiles<HD>(), TC = 64 * CT;
+__global__ __launch_bounds__(kBlock, HD == 256 ? 2 : 3) void kv4_attn_tile_kernel(const Kv4AttnArgs a) {
+    constexpr int DPL = HD / 16, CT = kColTiles, TC = 64 * CT;
     // the wavefronts' query parts at first, then the values of two blocks
     constexpr size_t PARTS = 4 * sizeof(Kv4SharedQuery<HD>), VALUES = 4 * DPL * 64 * sizeof(u32x4);
     __shared__ __attribute__((aligned(16))) char s_buf[PARTS > VALUES ? PARTS : VALUES];
@@ -1139,7 +1138,7 @@ __global__ __launch_bounds__(kBlock, 2) void kv4_attn_tile_kernel(const Kv4AttnA
 Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq) {
     Kv4Plan p{};
     const int64_t ncol = (int64_t)rows * (nq / c.nkv);
-    const int tc = 64 * (c.hd == 256 ? kv4_col_tiles<256>() : kv4_col_tiles<128>());
+    const int tc = 64 * kColTiles;
     p.ntile = (int)((ncol + tc - 1) / tc);
     p.items = (int64_t)p.ntile * c.n_seq;
     p.runs = 1;

@@ -427,9 +427,12 @@ constexpr int kKv4WholeBlocks = 2;    // blocks that one workgroup takes rather 
 // workspace.
 constexpr size_t kKv4CounterBytes = kKv4Workgroups * 4;
 // More columns (query rows x heads of a KV head) of a sequence than kKv4RowCols
-// take the tile kernel, where its tiles are enough workgroups to fill the chip.
+// take the tile kernel, where its tiles are kKv4TileWorkgroups workgroups or
+// more: 16 heads over 8 of 128, 1000 / 2000 / 4000 tokens (256 / 504 / 1000
+// tiles) 40 / 74 / 155 us against the rows kernel's 30 / 73 / 208, 2000 tokens
+// after 6000 283 against 314.
 constexpr int kKv4RowCols = 32;
-constexpr int64_t kKv4TileWorkgroups = 256;
+constexpr int64_t kKv4TileWorkgroups = 500;
 struct Kv4Plan {
     bool tile;      // the tile kernel, else the rows kernel
     int part_cols;  // columns of an item's partial states

@@ -309,6 +309,35 @@ def test_attn_long_prompt(T, H):
         check_attn(c, got[:, t:t + 1], q[:, t:t + 1], [71 + t])
 
 
+@pytest.mark.parametrize("hd", [16, 32, 64, 128, 256])
+def test_attn_prompts_with_values_of_all_sizes(T, H, hd):
+    """Sequences of values around 1, growing by 2^60 within a block of keys and
+    between blocks, shrinking, with zeros, and of 2^-60 only."""
+    rng = np.random.default_rng(hd)
+    c = Cache(T, H, 400, 4, hd, n_seq=128)
+    size = np.zeros((128, 400))
+    size[1] = np.repeat([-60, -30, 0, 5, 30, 60, 20, -20], 50)
+    size[2] = rng.integers(-12, 13, 400)
+    size[3] = rng.integers(-60, 61, 400)
+    size[4] = -60
+    size[5] = np.linspace(60, -60, 400)
+    size[6] = np.where(np.arange(400) % 100 < 70, -40, 40)
+    size[7] = np.where(np.arange(400) < 200, -110, 0)
+
+    def sized(v):
+        v = (v * np.exp2(size)[..., None, None]).astype(np.float32)
+        v[8, 100:300] = 0.0
+        v[9] = 0.0
+        v[6, 150, 0, 0] = np.inf
+        return v
+    c.fill(rng, 400, values=sized)
+    q = rng.standard_normal((128, 36, 8, hd)).astype(np.float32)
+    pos = [364] * 128
+    pos[1], pos[6] = 300, 130
+    got = attend(c, q, pos, dev=ints(H, pos))
+    check_attn(c, got, q, pos, only=range(12))
+
+
 def test_attn_sharp_and_flat_softmax(T, H):
     """Scores of some hundreds, one dominant key, and equal keys."""
     rng = np.random.default_rng(9)
@@ -441,6 +470,19 @@ def test_attn_large_and_small_magnitudes(T, H):
            keys=lambda k: (k * np.exp2(rng.integers(-6, 4, (1, 260, 1, 1)))).astype(np.float32))
     q = rng.standard_normal((1, 2, 4, 128)).astype(np.float32)
     check_attn(c, attend(c, q, [258]), q, [258])
+
+
+def test_host_memory_is_refused(T, H):
+    """Before anything is launched."""
+    from tinyminigo_amd._lib import TMG_E_INVALID
+    host = np.zeros(T.kv4_bytes(64, 2, 64) + 16, np.uint8)
+    kv = T.Kv4((host.ctypes.data + 15) // 16 * 16, cap=64, nkv=2, hd=64)
+    dev = H.DeviceBuffer(1 << 16)
+    for call in (lambda: T.kv4_write(kv, dev.addr, dev.addr, 1), lambda: T.kv4_read(kv, dev.addr, dev.addr, 1),
+                 lambda: T.kv4_attn(kv, dev.addr, dev.addr + 4096, 1, 4)):
+        with pytest.raises(T.TmgError) as e:
+            call()
+        assert e.value.code == TMG_E_INVALID
 
 
 def test_attn_on_a_stream_and_in_graphs(T, H):

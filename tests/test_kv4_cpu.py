@@ -120,6 +120,22 @@ def test_attn_nothing_to_do():
     assert lib.tmg_kv4_attn(C.byref(kv()), None, None) == TMG_E_INVALID
 
 
+def test_too_many_rows_for_one_call():
+    c = kv(cap=1 << 30, nkv=1, hd=256, n_seq=1)
+    assert rows_call(lib.tmg_kv4_write, c, rows=(1 << 26) + 1) == TMG_E_INVALID
+    assert attn(kv(cap=1 << 26, nkv=1, hd=16, n_seq=1), rows=1 << 26, nq=4, pos=0) == TMG_E_INVALID
+
+
+def test_valid_calls_without_a_device():
+    from tinyminigo_amd import hip as H
+    from tinyminigo_amd._lib import TMG_E_DEVICE
+    if H.device_count():
+        pytest.skip("needs a machine without a GPU")
+    assert rows_call(lib.tmg_kv4_write, kv()) == TMG_E_DEVICE
+    assert rows_call(lib.tmg_kv4_read, kv()) == TMG_E_DEVICE
+    assert attn(kv()) == TMG_E_DEVICE
+
+
 def test_workspace_covers_every_position():
     # what a call at any position needs is within what the workspace query says
     for rows, nq, nkv, hd, cap, n_seq in [(1, 16, 8, 128, 131072, 1), (45, 16, 8, 128, 8192, 1), (1, 32, 8, 128, 4096, 48),

@@ -23,7 +23,8 @@ class StreamDevice {
         if (s && hipStreamGetDevice(s, &dev) != hipSuccess) return device_error("bad stream");
         hipPointerAttribute_t at;
         memset(&at, 0, sizeof(at));
-        if (hipPointerGetAttributes(&at, data) != hipSuccess) {
+        if (hipPointerGetAttributes(&at, data) != hipSuccess ||
+            (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged)) {
             (void)hipGetLastError();
             return set_error(TMG_E_INVALID, "the cache is not in device memory");
         }
@@ -69,6 +70,8 @@ int check_cache(const tmg_kv4 *kv, uint32_t rows, const int32_t *pos_dev, uint32
     if (kv->n_seq > 1 && kv->seq_stride < kv4_slab_bytes(kv->cap, (int)kv->nkv, (int)kv->hd))
         return set_error(TMG_E_INVALID, "sequence stride below a sequence's bytes");
     if ((uintptr_t)pos_dev & 3) return set_error(TMG_E_INVALID, "positions must be 4-byte aligned");
+    // a launch has fewer than 2^32 threads along a dimension
+    if ((uint64_t)rows * (kv->hd / 8) > 1u << 31) return set_error(TMG_E_INVALID, "too many rows for one call");
     if (rows > kv->cap || (!pos_dev && (uint64_t)pos + rows > kv->cap))
         return set_error(TMG_E_CAPACITY, "rows past the 4-bit cache's capacity (" + std::to_string(kv->cap) + " positions)");
     return TMG_OK;
@@ -130,9 +133,9 @@ namespace {
 int check_heads(const tmg_kv4 *kv, uint32_t rows, uint32_t nq) {
     if (nq == 0 || nq % kv->nkv != 0 || nq > 65536)
         return set_error(TMG_E_INVALID, "query heads must be a multiple of the KV heads");
-    // columns and workgroups stay within 31 bits
+    // columns stay within 31 bits, and the threads of 256 for 16 of them
     const uint64_t ncol = (uint64_t)rows * (nq / kv->nkv);
-    if (ncol > 0x7ffffff0u || (ncol + 15) / 16 * kv->nkv * kv->n_seq > 0x7fffffffu)
+    if (ncol > 0x7ffffff0u || (ncol + 15) / 16 * kv->nkv * kv->n_seq > 1u << 23)
         return set_error(TMG_E_INVALID, "too many query rows for one call");
     return TMG_OK;
 }

@@ -244,6 +244,23 @@ __device__ __forceinline__ void kv4_scores(const Kv4Key<HD> (&k)[TILES], const K
         for (int e = 0; e < 4; e++) s[i][e] = Kv4Lanes<C>::sum(s[i][e]);
 }
 
+// Whether a lane of the wavefront has a scale byte past the largest; those are
+// replaced then, and *bits tells the lane's.
+__device__ __forceinline__ bool take_marks(uint32_t (&scale)[8], uint32_t *bits) {
+    uint32_t most = scale[0];
+#pragma unroll
+    for (int j = 1; j < 8; j++) most = max(most, scale[j]);
+    *bits = 0;
+    if (__builtin_amdgcn_ballot_w64(most > kKv4MaxScale) == 0) return false;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const bool marked = scale[j] > kKv4MaxScale;
+        *bits |= marked ? 1u << j : 0u;
+        scale[j] = marked ? 127u : scale[j];
+    }
+    return true;
+}
+
 // A lane's HD / 16 dimensions of its eight keys of a unit of 32.
 template <int HD>
 struct Kv4Values {
@@ -252,11 +269,12 @@ struct Kv4Values {
     uint32_t code[8][W];
     uint32_t scale[8];
 
-    // Row d and those after it repeat row d of the planes' first 32.
+    // Rows 0 .. 31 of the planes; unless WHOLE, rows past d repeat row d.
+    template <bool WHOLE>
     __device__ __forceinline__ void load(const uint8_t *vc, const uint8_t *vs, int d, int r, int lg) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const unsigned row = (unsigned)min(16 * (j >> 2) + 4 * lg + (j & 3), d);
+            const unsigned at = 16 * (j >> 2) + 4 * lg + (j & 3), row = WHOLE ? at : min(at, (unsigned)d);
             const uint8_t *p = vc + row * (HD / 2);
             if constexpr (HD == 256) {
                 const uint2 c = *reinterpret_cast<const uint2 *>(p + 8 * r);
@@ -279,18 +297,7 @@ struct Kv4Values {
     // values are then taken as finite ones (a masked key's weight of zero
     // must not meet a NaN), and nan_values puts the NaN where it belongs.  So
     // do the scales past the largest, which only rows never written can hold.
-    __device__ __forceinline__ bool take_bad(uint32_t *bits) {
-        uint32_t b = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if (scale[j] > kKv4MaxScale) {
-                b |= 1u << j;
-                scale[j] = 127;
-            }
-        }
-        *bits = b;
-        return __builtin_amdgcn_ballot_w64(b != 0) != 0;
-    }
+    __device__ __forceinline__ bool take_bad(uint32_t *bits) { return take_marks(scale, bits); }
 
     // The bf16 operands of two neighbouring tiles: dimensions 2 i and 2 i + 1
     // of the lane's, eight keys each.
@@ -530,14 +537,18 @@ __device__ __forceinline__ Kv4Item kv4_item(const Kv4AttnArgs &a, int i) {
     return kv4_item<BLOCK>(a, i, a.pos_dev ? a.pos_dev[a.ntile == 1 ? i : i / a.ntile] : a.pos);
 }
 
-// Output element d of the item's column c.
+// Output elements d, d + 1 of the item's column c.
 template <int HD>
-__device__ __forceinline__ void kv4_put(const Kv4AttnArgs &a, const Kv4Item &it, int g, int c, int d, float O, float L) {
+__device__ __forceinline__ void kv4_put(const Kv4AttnArgs &a, const Kv4Item &it, int g, int c, int d, float2 O, float L) {
     const int dt = div_group(a, it.h0 + c), h = it.h0 + c - dt * a.group;
     const size_t i = ((size_t)it.seq * a.rows + it.t0 + dt) * a.out_stride + (size_t)(g * a.group + h) * HD + d;
-    const float v = L == 0.f ? 0.f : O * __builtin_amdgcn_rcpf(L);  // (the reciprocal is within an ulp)
-    if (a.out) a.out[i] = v;
-    if (a.out_hi) split_bf16(v, a.out_hi + i, a.out_lo + i);
+    const float f = L == 0.f ? 0.f : __builtin_amdgcn_rcpf(L);  // (within an ulp)
+    const float x = O.x * f, y = O.y * f;
+    if (a.out) *reinterpret_cast<float2 *>(a.out + i) = make_float2(x, y);
+    if (a.out_hi) {
+        split_bf16(x, a.out_hi + i, a.out_lo + i);
+        split_bf16(y, a.out_hi + i + 1, a.out_lo + i + 1);
+    }
 }
 
 // Wavefronts of a workgroup; a wavefront takes 32 keys of a block.  One item
@@ -583,7 +594,7 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
     __shared__ unsigned s_arrived;
     __shared__ int s_first[ONE ? 1 : kKv4FlatItems + 1];  // the items' first blocks in the row of all
     __shared__ int s_sum[NW], s_start;
-    __shared__ float s_red[NT];
+    __shared__ float2 s_red[NT];
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r = lane & 15, lg = lane >> 4;
     // (run, KV head): one item's runs read different keys; several items' tiles
     // share a head's, whose workgroups are nkv apart, so on one XCD for eight
@@ -604,9 +615,16 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
         const int at = min(key0, lim), d = lim - at;
         const size_t row = row0 + at;
         const uint8_t *const kc = pl.kc + row * (HD / 2), *const ks = pl.ks + row * kv4_groups(HD);
-        k[0].load(kc, ks, (unsigned)min(r, d), lg);
-        k[1].load(kc, ks, (unsigned)min(16 + r, d), lg);
-        v.load(pl.vc + row * (HD / 2), pl.vs + row * kv4_groups(HD), d, r, lg);
+        const uint8_t *const vc = pl.vc + row * (HD / 2), *const vs = pl.vs + row * kv4_groups(HD);
+        if (d >= 31) {  // constant offsets: a third of the unit's address arithmetic
+            k[0].load(kc, ks, (unsigned)r, lg);
+            k[1].load(kc, ks, (unsigned)(16 + r), lg);
+            v.template load<true>(vc, vs, d, r, lg);
+        } else {
+            k[0].load(kc, ks, (unsigned)min(r, d), lg);
+            k[1].load(kc, ks, (unsigned)min(16 + r, d), lg);
+            v.template load<false>(vc, vs, d, r, lg);
+        }
     };
     auto fetch = [&](int seq, int t0, int h0, int cols) {
         const int c = h0 + min(rc, cols - 1), dt = div_group(a, c), h = c - dt * a.group;
@@ -786,31 +804,32 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
         // partial states: two slots a run, the second for an item that the
         // run begins after another
         const size_t slot = ((size_t)g * a.runs + run) * 2 + (begun ? 1 : 0);
-        for (int idx = t; idx < cols * HD; idx += NT) {
-            const int c = idx / HD, d = idx % HD;
+        for (int idx = t; idx < cols * (HD / 2); idx += NT) {
+            const int c = idx / (HD / 2), d = idx % (HD / 2) * 2;
             float M = s_m[c][0];
 #pragma unroll
             for (int w = 1; w < NW; w++) M = fmaxf(M, s_m[c][w]);
-            float L = 0.f, O = 0.f;
+            float L = 0.f;
+            float2 O = make_float2(0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < NW; w++) {
                 // a wavefront without a finite maximum still brings its sums:
                 // they are zeros, or NaN
                 const float f = s_m[c][w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[c][w] - M);
                 L = fmaf(s_l[c][w], f, L);
-                float sum = s_o[(w * 16 + c * PARTS) * PITCH + d];
+                float2 sum = *reinterpret_cast<const float2 *>(s_o + (w * 16 + c * PARTS) * PITCH + d);
 #pragma unroll
-                for (int e = 1; e < OPARTS; e++) sum += s_o[(w * 16 + c * PARTS + e) * PITCH + d];
-                O = fmaf(sum, f, O);
+                for (int e = 1; e < OPARTS; e++) {
+                    const float2 x = *reinterpret_cast<const float2 *>(s_o + (w * 16 + c * PARTS + e) * PITCH + d);
+                    sum = make_float2(sum.x + x.x, sum.y + x.y);
+                }
+                O = make_float2(fmaf(sum.x, f, O.x), fmaf(sum.y, f, O.y));
             }
             if (parts == 1) {
                 kv4_put<HD>(a, it, g, c, d, O, L);
             } else {
-                st_dev(a.part + (slot * a.part_cols + c) * HD + d, O);
-                if (d == 0) {
-                    st_dev(a.part_ml + (slot * a.part_cols + c) * 2, M);
-                    st_dev(a.part_ml + (slot * a.part_cols + c) * 2 + 1, L);
-                }
+                st_dev2(a.part + (slot * a.part_cols + c) * HD + d, O.x, O.y);
+                if (d == 0) st_dev2(a.part_ml + (slot * a.part_cols + c) * 2, M, L);
             }
         }
         if (parts > 1) {
@@ -828,19 +847,20 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
                 const bool late0 = flat && r0 * per < s_first[item];
                 const size_t slot0 = ((size_t)g * a.runs + r0) * 2;
                 auto part = [&](int i) { return (slot0 + 2 * (size_t)i + (i == 0 && late0 ? 1 : 0)) * a.part_cols; };
-                // SUB threads an element, each with the parts sub, sub + SUB,
-                // ..; its first parts are on their way while the columns'
+                // SUB threads a pair of elements, each with the parts sub, sub +
+                // SUB, ..; its first parts are on their way while the columns'
                 // weights and sums are made
-                constexpr int FAR = kKv4MaxRuns / 64, AHEAD = 16;
-                const int elems = cols * HD, SUB = max(1, NT / elems);
-                const int e0 = SUB == 1 ? t : t % elems, sub = SUB == 1 ? 0 : t / elems;
-                float ahead[AHEAD];
+                constexpr int FAR = kKv4MaxRuns / 64, AHEAD = C == 16 ? 8 : 16;
+                const int pairs = cols * (HD / 2), SUB = max(1, NT / pairs);
+                const int e0 = SUB == 1 ? t : t % pairs, sub = SUB == 1 ? 0 : t / pairs;
+                float2 ahead[AHEAD];
                 auto grab = [&](int e, int i) {
-                    const float *src = a.part + (size_t)(e / HD) * HD + e % HD;
+                    const float *src = a.part + (size_t)(e / (HD / 2)) * HD + e % (HD / 2) * 2;
 #pragma unroll
-                    for (int u = 0; u < AHEAD; u++) ahead[u] = ld_dev(src + part(min(i + u * SUB, parts - 1)) * HD);
+                    for (int u = 0; u < AHEAD; u++)
+                        if (i + u * SUB < parts) ahead[u] = ld_dev2(src + part(i + u * SUB) * HD);
                 };
-                const bool busy = sub < SUB && e0 < elems;
+                const bool busy = sub < SUB && e0 < pairs;
                 if (busy) grab(e0, sub);
                 for (int c = wave; c < cols; c += NW) {
                     float M = -INFINITY, L = 0.f, m[FAR], l[FAR];
@@ -849,9 +869,9 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
                         m[i] = -INFINITY;
                         l[i] = 0.f;
                         if (64 * i >= parts) continue;
-                        const float *ml = a.part_ml + (part(min(lane + 64 * i, parts - 1)) + c) * 2;
-                        m[i] = ld_dev(ml);
-                        l[i] = ld_dev(ml + 1);
+                        const float2 ml = ld_dev2(a.part_ml + (part(min(lane + 64 * i, parts - 1)) + c) * 2);
+                        m[i] = ml.x;
+                        l[i] = ml.y;
                     }
 #pragma unroll
                     for (int i = 0; i < FAR; i++) M = fmaxf(M, m[i]);
@@ -869,27 +889,30 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
                 }
                 __syncthreads();
                 bool fresh = true;
-                for (int e = e0; busy && e < elems; e += NT) {
-                    const int c = e / HD;
-                    float O = 0.f;
+                for (int e = e0; busy && e < pairs; e += NT) {
+                    const int c = e / (HD / 2);
+                    float2 O = make_float2(0.f, 0.f);
                     for (int i = sub; i < parts; i += AHEAD * SUB) {
                         if (!fresh) grab(e, i);
                         fresh = false;
 #pragma unroll
                         for (int u = 0; u < AHEAD; u++)
-                            if (i + u * SUB < parts) O = fmaf(ahead[u], s_o[c * kKv4MaxRuns + i + u * SUB], O);
+                            if (i + u * SUB < parts) {
+                                const float f = s_o[c * kKv4MaxRuns + i + u * SUB];
+                                O = make_float2(fmaf(ahead[u].x, f, O.x), fmaf(ahead[u].y, f, O.y));
+                            }
                     }
                     if (SUB == 1)
-                        kv4_put<HD>(a, it, g, c, e % HD, O, s_l[c][0]);
+                        kv4_put<HD>(a, it, g, c, e % (HD / 2) * 2, O, s_l[c][0]);
                     else
-                        s_red[sub * elems + e] = O;
+                        s_red[sub * pairs + e] = O;
                 }
                 if (SUB > 1) {
                     __syncthreads();
-                    if (t < elems) {
-                        float O = s_red[t];
-                        for (int i = 1; i < SUB; i++) O += s_red[i * elems + t];
-                        kv4_put<HD>(a, it, g, t / HD, t % HD, O, s_l[t / HD][0]);
+                    if (t < pairs) {
+                        float2 O = s_red[t];
+                        for (int i = 1; i < SUB; i++) O = make_float2(O.x + s_red[i * pairs + t].x, O.y + s_red[i * pairs + t].y);
+                        kv4_put<HD>(a, it, g, t / (HD / 2), t % (HD / 2) * 2, O, s_l[t / (HD / 2)][0]);
                     }
                 }
             }
@@ -914,10 +937,11 @@ struct Kv4Stage {
     static constexpr int DPL = HD / 16, TILES = DPL < 4 ? DPL : DPL / 2;
     uint32_t code[8], scale[8];
 
+    template <bool WHOLE>
     __device__ __forceinline__ void load(const uint8_t *vc, const uint8_t *vs, int d, int half, int r, int lg) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const unsigned row = (unsigned)min(16 * (j >> 2) + 4 * lg + (j & 3), d);
+            const unsigned at = 16 * (j >> 2) + 4 * lg + (j & 3), row = WHOLE ? at : min(at, (unsigned)d);
             const uint8_t *p = vc + row * (HD / 2);
             if constexpr (HD == 256)
                 code[j] = *reinterpret_cast<const uint32_t *>(p + 8 * r + 4 * half);
@@ -934,14 +958,8 @@ struct Kv4Stage {
     // The tiles' bf16 operands to dst[tile][64 lanes]; the marked lanes of
     // each key to mark, and whether there are any to *any (by half 0).
     __device__ __forceinline__ void store(u32x4 (*dst)[64], unsigned long long *mark, int *any, int half, int lane) {
-        uint32_t bad = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (scale[j] > kKv4MaxScale) {
-                bad |= 1u << j;
-                scale[j] = 127;
-            }
-        const bool some = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+        uint32_t bad;
+        const bool some = take_marks(scale, &bad);
         if (half == 0) {
             if (some) {
 #pragma unroll
@@ -1029,14 +1047,23 @@ __global__ __launch_bounds__(kBlock, HD == 256 ? 2 : 3) void kv4_attn_tile_kerne
     auto load_keys = [&](int key0) {
         const int at = min(key0, last), d = last - at;
         const size_t row = row0 + at;
+        const uint8_t *const kc = pl.kc + row * (HD / 2), *const ks = pl.ks + row * kv4_groups(HD);
+        if (d >= kTileKeys - 1) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            k[i].load(pl.kc + row * (HD / 2), pl.ks + row * kv4_groups(HD), (unsigned)min(16 * i + r, d), lg);
+            for (int i = 0; i < 4; i++) k[i].load(kc, ks, (unsigned)(16 * i + r), lg);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) k[i].load(kc, ks, (unsigned)min(16 * i + r, d), lg);
+        }
     };
     auto load_values = [&](int key0) {
         const int at = min(key0 + 32 * unit, last);
         const size_t row = row0 + at;
-        v.load(pl.vc + row * (HD / 2), pl.vs + row * kv4_groups(HD), last - at, half, r, lg);
+        const uint8_t *const vc = pl.vc + row * (HD / 2), *const vs = pl.vs + row * kv4_groups(HD);
+        if (last - at >= 31)
+            v.template load<true>(vc, vs, 31, half, r, lg);
+        else
+            v.template load<false>(vc, vs, last - at, half, r, lg);
     };
     if (nb) {
         load_keys(0);

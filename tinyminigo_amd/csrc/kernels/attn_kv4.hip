@@ -537,6 +537,70 @@ __device__ __forceinline__ Kv4Item kv4_item(const Kv4AttnArgs &a, int i) {
     return kv4_item<BLOCK>(a, i, a.pos_dev ? a.pos_dev[a.ntile == 1 ? i : i / a.ntile] : a.pos);
 }
 
+__device__ __forceinline__ float uniform(float v) {
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
+}
+
+// Shares a.runs workgroups of a KV head out to the items: an item of n blocks
+// gets ceil(n / each) of them, with the smallest `each` (to a 32nd of where it
+// can be) for which there are enough, so every workgroup has one item and most
+// have as many blocks.  Every wavefront finds its workgroup's share by itself;
+// all of them come to the same numbers.  False where workgroup `run` has none.
+template <int BLOCK>
+__device__ __forceinline__ bool kv4_deal(const Kv4AttnArgs &a, int run, int lane, int *item, int *part, int *parts) {
+    constexpr int PER = kKv4FlatItems / 64;  // items of a lane: 64 i + lane
+    float n[PER], total = 0.f, most = 1.f;   // (integers below 2^24)
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        if (64 * i >= a.items) continue;
+        n[i] = 64 * i + lane < a.items ? (float)max(1, kv4_item<BLOCK>(a, 64 * i + lane).nb) : 0.f;
+        total += n[i];
+        most = fmaxf(most, n[i]);
+    }
+    total = uniform(wave_sum(total));
+    most = uniform(wave_max(most));
+    float inv = 0.f;  // 1 / each
+    auto share = [&](float n) { return n > 0.f ? min((int)((n - 0.5f) * inv) + 1, kKv4MaxRuns) : 0; };
+    int lo = max((int)ceilf(total / (float)a.runs), max((int)most / kKv4MaxRuns, kKv4WholeKeys / BLOCK)), hi = max(lo, (int)most);
+    // one an item, and one more for every `each` blocks past the first
+    if (a.runs > a.items) hi = min(hi, max(lo, (int)((total - (float)a.items) / (float)(a.runs - a.items)) + 1));
+#pragma unroll 1
+    for (int turn = 0; turn < 5 && lo < hi; turn++) {
+        const int mid = (lo + hi) >> 1;
+        inv = __builtin_amdgcn_rcpf((float)mid);
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (64 * i < a.items) sum += share(n[i]);
+        if ((int)uniform(wave_sum((float)sum)) <= a.runs) hi = mid;
+        else lo = mid + 1;
+    }
+    inv = __builtin_amdgcn_rcpf((float)hi);
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        if (64 * i >= a.items) continue;
+        const int mine = share(n[i]);
+        int upto = mine;  // over the lanes up to this one
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int o = __shfl_up(upto, off, 64);
+            upto += lane >= off ? o : 0;
+        }
+        const int first = before + upto - mine;
+        const unsigned long long here = __builtin_amdgcn_ballot_w64(run >= first && run < first + mine);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            *item = 64 * i + l;
+            *part = run - __builtin_amdgcn_readlane(first, l);
+            *parts = __builtin_amdgcn_readlane(mine, l);
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
 // Output elements d, d + 1 of the item's column c.
 template <int HD>
 __device__ __forceinline__ void kv4_put(const Kv4AttnArgs &a, const Kv4Item &it, int g, int c, int d, float2 O, float L) {
@@ -561,20 +625,18 @@ constexpr int kv4_waves() {
     return ONE && HD < 256 ? 8 : 4;
 }
 
-// A workgroup owns one KV head and a run of blocks (32 keys a wavefront), each
+// A workgroup owns one KV head and blocks of an item (32 keys a wavefront), each
 // wavefront with a softmax state of its own; the wavefronts are merged through
-// LDS.  Where an item's blocks are dealt to several workgroups, the last of
-// them to arrive merges their states, in the order of the runs, so that the
-// result does not depend on who is last: one launch in all.
+// LDS.  Where several workgroups share an item they take its blocks in turn,
+// and the last of them to arrive merges their states, in the order of the
+// parts, so that the result does not depend on who is last: one launch in all.
 //
-// - ONE item: the workgroups take the blocks in turn.  A workgroup's first
-//   block does not hang on the position, so its keys are loaded before the
-//   position, which may live on the device, is known.
-// - Up to kKv4FlatItems items (a.flat): the items' blocks, one after the other, are cut
-//   into equal runs, whatever the sequences' lengths are; a run ends in the
-//   middle of an item and goes on with the next.  (The same number of
-//   workgroups for every item left sequences of 65 to 131070 positions at 100
-//   us, 1.9 times the time of their mean.)
+// - ONE item: a workgroup's first block does not hang on the position, so its
+//   keys are loaded before the position, which may live on the device, is
+//   known.
+// - Up to kKv4FlatItems items (a.flat): kv4_deal shares the workgroups out.
+//   (The same number of them for every item left sequences of 65 to 131070
+//   positions at 100 us, 1.9 times the time of their mean.)
 // - More items: a workgroup each.
 //
 // With a.k_new (one row a sequence) the wavefront that owns the new position
@@ -592,8 +654,6 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
     __shared__ Kv4SharedQuery<C == 16 ? HD : 16> s_q;
     __shared__ Kv4NewRow<HD> s_new;
     __shared__ unsigned s_arrived;
-    __shared__ int s_first[ONE ? 1 : kKv4FlatItems + 1];  // the items' first blocks in the row of all
-    __shared__ int s_sum[NW], s_start;
     __shared__ float2 s_red[NT];
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r = lane & 15, lg = lane >> 4;
     // (run, KV head): one item's runs read different keys; several items' tiles
@@ -660,8 +720,7 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
     };
 
     int pos0 = a.pos;
-    int item = 0, x = 0, xend = 1;  // blocks [x, xend) of all the items'
-    int per = 1, total = 0;         // blocks of a run, of all items
+    int item = 0, part = 0, parts = 1;  // this workgroup's, and those that share the item
     const bool flat = !ONE && a.flat;
     if constexpr (ONE) {
         // the query first: it is split while the first keys are on their way
@@ -676,265 +735,184 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
 #pragma unroll
                 for (int set = 0; set < Kv4Lanes<C>::QSETS; set++) asm volatile("" : "+v"(q.part[h][set]));
     } else if (flat) {
-        constexpr int PER = (kKv4FlatItems + NT - 1) / NT;
-        int n[PER], sum = 0;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            n[i] = t * PER + i < a.items ? max(1, kv4_item<BLOCK>(a, t * PER + i).nb) : 0;
-            sum += n[i];
-        }
-        int before = sum;  // over the wavefront's lanes up to this one
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int o = __shfl_up(before, off, 64);
-            before += lane >= off ? o : 0;
-        }
-        if (lane == 63) s_sum[wave] = before;
-        before -= sum;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < NW; w++) {
-            const int o = s_sum[w];
-            before += w < wave ? o : 0;
-            total += o;
-        }
-        total = __builtin_amdgcn_readfirstlane(total);
-        per = (int)(((unsigned)total + (unsigned)a.runs - 1) / (unsigned)a.runs);
-        if ((int64_t)run * per >= total) return;
-        x = run * per;
-        xend = min(x + per, total);
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            if (t * PER + i <= a.items) s_first[t * PER + i] = before;
-            if (x >= before && x < before + n[i]) s_start = t * PER + i;
-            before += n[i];
-        }
-        if (t == 0) s_first[a.items] = total;
-        __syncthreads();
-        item = __builtin_amdgcn_readfirstlane(s_start);
+        if (!kv4_deal<BLOCK>(a, run, lane, &item, &part, &parts)) return;
     } else {
         item = a.items - 1 - run;  // the latest rows, with the most keys, first
     }
-    const int x_begin = x, item0 = item;
-    Kv4Item it = ONE ? kv4_item<BLOCK>(a, 0, pos0) : kv4_item<BLOCK>(a, item);
-    for (; x < xend; item++) {
-        const Kv4Planes<HD> pl(a.c, it.seq);
-        // this workgroup's blocks b, b + step, .. < bend of the item, which
-        // `parts` workgroups share, the first of them run r0
-        int b = 0, bend = it.nb, step = 1, parts = 1, r0 = run;
-        bool begun = false;  // the run begins the item after another
-        if constexpr (ONE) {
-            if (it.nb > kKv4WholeBlocks) {
-                const unsigned each = ((unsigned)it.nb + a.runs - 1) / (unsigned)a.runs;
-                parts = (int)(((unsigned)it.nb + each - 1) / each);
-            }
-            if (run >= parts) return;
-            b = run;
-            step = parts;
-            r0 = 0;
-        } else if (flat) {
-            const int first = __builtin_amdgcn_readfirstlane(s_first[item]);
-            const int next = __builtin_amdgcn_readfirstlane(s_first[item + 1]);
-            b = x - first;
-            bend = min(min(xend, next) - first, it.nb);
-            if (x > first || xend < next) {
-                r0 = (int)((unsigned)first / (unsigned)per);
-                parts = (int)((unsigned)(next - 1) / (unsigned)per) - r0 + 1;
-                begun = x_begin < first;
-            }
-            x = min(xend, next);
+    const Kv4Item it = ONE ? kv4_item<BLOCK>(a, 0, pos0) : kv4_item<BLOCK>(a, item);
+    const Kv4Planes<HD> pl(a.c, it.seq);
+    if constexpr (ONE) {
+        if (it.nb > kKv4WholeKeys / BLOCK) {
+            const unsigned each = ((unsigned)it.nb + a.runs - 1) / (unsigned)a.runs;
+            parts = (int)(((unsigned)it.nb + each - 1) / each);
         }
-        if (!flat) xend = 0;
-        // the next item's position, read while this one's keys are
-        int pos_next = a.pos;
-        if (!ONE && a.pos_dev && x < xend) pos_next = a.pos_dev[a.ntile == 1 ? item + 1 : (item + 1) / a.ntile];
-        const int cols = it.cols, pos = it.pos;
-        Kv4State<HD> st;
-        if (pos >= 0) {
-            // (lanes past the columns repeat the last one)
-            const int qpos = pos + it.t0 + div_group(a, it.h0 + min(rc, cols - 1));
-            const int first_pos = pos + it.t0;
-            int key0 = b * BLOCK + 32 * wave;
-            const int end = min(bend * BLOCK, it.last + 1);
-            if constexpr (!ONE) {
-                if (C == 16 || item == item0) {
-                    fetch(it.seq, it.t0, it.h0, cols);
-                    load(pl, key0, it.last);
+        if (run >= parts) return;
+        part = run;
+    }
+    const int cols = it.cols, pos = it.pos;
+    Kv4State<HD> st;
+    if (pos >= 0) {
+        // (lanes past the columns repeat the last one)
+        const int qpos = pos + it.t0 + div_group(a, it.h0 + min(rc, cols - 1));
+        const int first_pos = pos + it.t0;
+        const int step = parts * BLOCK;
+        int key0 = part * BLOCK + 32 * wave;
+        if constexpr (!ONE) {
+            fetch(it.seq, it.t0, it.h0, cols);
+            load(pl, key0, it.last);
+            split(cols);
+        }
+        for (; key0 <= it.last; key0 += step) {
+            if (append && key0 + 31 >= pos) {
+                s_new.put(xn, lane, pl, row0 + pos);
+                // the wavefront's own LDS writes, in order
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                s_new.patch(k, v, pos - key0, r, lg);
+            }
+            f32x4 s[2];
+            kv4_scores(k, q, st.ref, pr, s);
+            Kv4Values<HD> vn = v;
+            if (key0 + step <= it.last) load(pl, key0 + step, it.last);
+            if (key0 + 31 > first_pos) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (key0 + 16 * (j >> 2) + 4 * lg + (j & 3) > qpos) s[j >> 2][j & 3] = -INFINITY;
+            }
+            float p[8];
+            st.weights(s, p);
+            bf16x8 pp[Kv4Lanes<C>::PSETS];
+            split_p<C>(p, pr, pp);
+            uint32_t bad;
+            const bool any_bad = vn.take_bad(&bad);
+            kv4_values(vn, pp, st.o);
+            if (any_bad)
+                nan_values<HD>([&](int j) { return __builtin_amdgcn_ballot_w64((bad >> j) & 1); }, key0, qpos, lg, st.o);
+        }
+    }
+    // the wavefronts' states
+    st.l = add_xor32(add_xor16(st.l));
+    constexpr int OPARTS = C < 16 ? kPParts : 1;  // lanes with parts of a column's sums
+    if (rc < cols && pr < OPARTS) {
+        float *const dst = s_o + (wave * 16 + r) * PITCH + 4 * lg * DPL;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int d = 0; d < DPL; d++) dst[i * DPL + d] = st.o[d][i];
+        if (lg == 0 && pr == 0) {
+            s_m[rc][wave] = st.max_ref();
+            s_l[rc][wave] = st.l;
+        }
+    }
+    lds_barrier();  // (an appended row's stores may still be on their way)
+    const size_t slot0 = (size_t)g * a.runs + run - part, slot = slot0 + part;  // of partial states
+    for (int idx = t; idx < cols * (HD / 2); idx += NT) {
+        const int c = idx / (HD / 2), d = idx % (HD / 2) * 2;
+        float M = s_m[c][0];
+#pragma unroll
+        for (int w = 1; w < NW; w++) M = fmaxf(M, s_m[c][w]);
+        float L = 0.f;
+        float2 O = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            // a wavefront without a finite maximum still brings its sums:
+            // they are zeros, or NaN
+            const float f = s_m[c][w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[c][w] - M);
+            L = fmaf(s_l[c][w], f, L);
+            float2 sum = *reinterpret_cast<const float2 *>(s_o + (w * 16 + c * PARTS) * PITCH + d);
+#pragma unroll
+            for (int e = 1; e < OPARTS; e++) {
+                const float2 x = *reinterpret_cast<const float2 *>(s_o + (w * 16 + c * PARTS + e) * PITCH + d);
+                sum = make_float2(sum.x + x.x, sum.y + x.y);
+            }
+            O = make_float2(fmaf(sum.x, f, O.x), fmaf(sum.y, f, O.y));
+        }
+        if (parts == 1) {
+            kv4_put<HD>(a, it, g, c, d, O, L);
+        } else {
+            st_dev2(a.part + (slot * a.part_cols + c) * HD + d, O.x, O.y);
+            if (d == 0) st_dev2(a.part_ml + (slot * a.part_cols + c) * 2, M, L);
+        }
+    }
+    if (parts > 1) {
+        // a workgroup's partial state is complete before it counts itself in
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        unsigned *const count = a.arrived + slot0;
+        if (t == 0) s_arrived = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (s_arrived == (unsigned)parts - 1) {
+            if (t == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            auto at = [&](int i) { return (slot0 + i) * a.part_cols; };
+            // SUB threads a pair of elements, each with the parts sub, sub +
+            // SUB, ..; its first parts are on their way while the columns'
+            // weights and sums are made
+            constexpr int FAR = kKv4MaxRuns / 64, AHEAD = C == 16 ? 8 : 16;
+            const int pairs = cols * (HD / 2), SUB = max(1, NT / pairs);
+            const int e0 = SUB == 1 ? t : t % pairs, sub = SUB == 1 ? 0 : t / pairs;
+            float2 ahead[AHEAD];
+            auto grab = [&](int e, int i) {
+                const float *src = a.part + (size_t)(e / (HD / 2)) * HD + e % (HD / 2) * 2;
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++)
+                    if (i + u * SUB < parts) ahead[u] = ld_dev2(src + at(i + u * SUB) * HD);
+            };
+            const bool busy = sub < SUB && e0 < pairs;
+            if (busy) grab(e0, sub);
+            for (int c = wave; c < cols; c += NW) {
+                float M = -INFINITY, L = 0.f, m[FAR], l[FAR];
+#pragma unroll
+                for (int i = 0; i < FAR; i++) {
+                    m[i] = -INFINITY;
+                    l[i] = 0.f;
+                    if (64 * i >= parts) continue;
+                    const float2 ml = ld_dev2(a.part_ml + (at(min(lane + 64 * i, parts - 1)) + c) * 2);
+                    m[i] = ml.x;
+                    l[i] = ml.y;
                 }
-                split(cols);
-            }
-            for (; key0 < end; key0 += step * BLOCK) {
-                if (append && key0 + 31 >= pos) {
-                    s_new.put(xn, lane, pl, row0 + pos);
-                    // the wavefront's own LDS writes, in order
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    __builtin_amdgcn_wave_barrier();
-                    s_new.patch(k, v, pos - key0, r, lg);
+#pragma unroll
+                for (int i = 0; i < FAR; i++) M = fmaxf(M, m[i]);
+                M = wave_max(M);
+#pragma unroll
+                for (int i = 0; i < FAR; i++) {
+                    if (64 * i >= parts) continue;
+                    const bool there = lane + 64 * i < parts;
+                    const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - M);
+                    L = there ? fmaf(l[i], f, L) : L;
+                    if (there) s_o[c * kKv4MaxRuns + lane + 64 * i] = f;
                 }
-                f32x4 s[2];
-                kv4_scores(k, q, st.ref, pr, s);
-                Kv4Values<HD> vn = v;
-                if (key0 + step * BLOCK < end) load(pl, key0 + step * BLOCK, it.last);
-                if (key0 + 31 > first_pos) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (key0 + 16 * (j >> 2) + 4 * lg + (j & 3) > qpos) s[j >> 2][j & 3] = -INFINITY;
-                }
-                float p[8];
-                st.weights(s, p);
-                bf16x8 pp[Kv4Lanes<C>::PSETS];
-                split_p<C>(p, pr, pp);
-                uint32_t bad;
-                const bool any_bad = vn.take_bad(&bad);
-                kv4_values(vn, pp, st.o);
-                if (any_bad)
-                    nan_values<HD>([&](int j) { return __builtin_amdgcn_ballot_w64((bad >> j) & 1); }, key0, qpos, lg, st.o);
+                L = wave_sum(L);
+                if (lane == 0) s_l[c][0] = L;
             }
-        }
-        // the wavefronts' states
-        st.l = add_xor32(add_xor16(st.l));
-        constexpr int OPARTS = C < 16 ? kPParts : 1;  // lanes with parts of a column's sums
-        if (rc < cols && pr < OPARTS) {
-            float *const dst = s_o + (wave * 16 + r) * PITCH + 4 * lg * DPL;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int d = 0; d < DPL; d++) dst[i * DPL + d] = st.o[d][i];
-            if (lg == 0 && pr == 0) {
-                s_m[rc][wave] = st.max_ref();
-                s_l[rc][wave] = st.l;
-            }
-        }
-        // the next item's query and first keys are on their way during the
-        // merge (48 ragged sequences 36.9 -> 36.0 us; with 16 columns a lane
-        // has no registers left for them)
-        Kv4Item it_next = it;
-        if (!ONE && x < xend) {
-            it_next = kv4_item<BLOCK>(a, item + 1, pos_next);
-            if (C < 16 && it_next.pos >= 0) {
-                fetch(it_next.seq, it_next.t0, it_next.h0, it_next.cols);
-                load(Kv4Planes<HD>(a.c, it_next.seq), 32 * wave, it_next.last);
-            }
-        }
-        lds_barrier();  // (an appended row's stores may still be on their way)
-        // partial states: two slots a run, the second for an item that the
-        // run begins after another
-        const size_t slot = ((size_t)g * a.runs + run) * 2 + (begun ? 1 : 0);
-        for (int idx = t; idx < cols * (HD / 2); idx += NT) {
-            const int c = idx / (HD / 2), d = idx % (HD / 2) * 2;
-            float M = s_m[c][0];
-#pragma unroll
-            for (int w = 1; w < NW; w++) M = fmaxf(M, s_m[c][w]);
-            float L = 0.f;
-            float2 O = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < NW; w++) {
-                // a wavefront without a finite maximum still brings its sums:
-                // they are zeros, or NaN
-                const float f = s_m[c][w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[c][w] - M);
-                L = fmaf(s_l[c][w], f, L);
-                float2 sum = *reinterpret_cast<const float2 *>(s_o + (w * 16 + c * PARTS) * PITCH + d);
-#pragma unroll
-                for (int e = 1; e < OPARTS; e++) {
-                    const float2 x = *reinterpret_cast<const float2 *>(s_o + (w * 16 + c * PARTS + e) * PITCH + d);
-                    sum = make_float2(sum.x + x.x, sum.y + x.y);
-                }
-                O = make_float2(fmaf(sum.x, f, O.x), fmaf(sum.y, f, O.y));
-            }
-            if (parts == 1) {
-                kv4_put<HD>(a, it, g, c, d, O, L);
-            } else {
-                st_dev2(a.part + (slot * a.part_cols + c) * HD + d, O.x, O.y);
-                if (d == 0) st_dev2(a.part_ml + (slot * a.part_cols + c) * 2, M, L);
-            }
-        }
-        if (parts > 1) {
-            // a workgroup's partial state is complete before it counts itself
-            // in; no other shared item starts in r0
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            unsigned *const count = a.arrived + (size_t)g * a.runs + r0;
-            if (t == 0) s_arrived = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __syncthreads();
-            if (s_arrived == (unsigned)parts - 1) {
-                if (t == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                // part i is run r0 + i, in its first slot but for a run that
-                // came to the item after another, which only r0 can
-                const bool late0 = flat && r0 * per < s_first[item];
-                const size_t slot0 = ((size_t)g * a.runs + r0) * 2;
-                auto part = [&](int i) { return (slot0 + 2 * (size_t)i + (i == 0 && late0 ? 1 : 0)) * a.part_cols; };
-                // SUB threads a pair of elements, each with the parts sub, sub +
-                // SUB, ..; its first parts are on their way while the columns'
-                // weights and sums are made (as many as leave the registers)
-                constexpr int FAR = kKv4MaxRuns / 64, AHEAD = C == 16 || !ONE ? 8 : 16;
-                const int pairs = cols * (HD / 2), SUB = max(1, NT / pairs);
-                const int e0 = SUB == 1 ? t : t % pairs, sub = SUB == 1 ? 0 : t / pairs;
-                float2 ahead[AHEAD];
-                auto grab = [&](int e, int i) {
-                    const float *src = a.part + (size_t)(e / (HD / 2)) * HD + e % (HD / 2) * 2;
+            bool fresh = true;
+            for (int e = e0; busy && e < pairs; e += NT) {
+                const int c = e / (HD / 2);
+                float2 O = make_float2(0.f, 0.f);
+                for (int i = sub; i < parts; i += AHEAD * SUB) {
+                    if (!fresh) grab(e, i);
+                    fresh = false;
 #pragma unroll
                     for (int u = 0; u < AHEAD; u++)
-                        if (i + u * SUB < parts) ahead[u] = ld_dev2(src + part(i + u * SUB) * HD);
-                };
-                const bool busy = sub < SUB && e0 < pairs;
-                if (busy) grab(e0, sub);
-                for (int c = wave; c < cols; c += NW) {
-                    float M = -INFINITY, L = 0.f, m[FAR], l[FAR];
-#pragma unroll
-                    for (int i = 0; i < FAR; i++) {
-                        m[i] = -INFINITY;
-                        l[i] = 0.f;
-                        if (64 * i >= parts) continue;
-                        const float2 ml = ld_dev2(a.part_ml + (part(min(lane + 64 * i, parts - 1)) + c) * 2);
-                        m[i] = ml.x;
-                        l[i] = ml.y;
-                    }
-#pragma unroll
-                    for (int i = 0; i < FAR; i++) M = fmaxf(M, m[i]);
-                    M = wave_max(M);
-#pragma unroll
-                    for (int i = 0; i < FAR; i++) {
-                        if (64 * i >= parts) continue;
-                        const bool there = lane + 64 * i < parts;
-                        const float f = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - M);
-                        L = there ? fmaf(l[i], f, L) : L;
-                        if (there) s_o[c * kKv4MaxRuns + lane + 64 * i] = f;
-                    }
-                    L = wave_sum(L);
-                    if (lane == 0) s_l[c][0] = L;
+                        if (i + u * SUB < parts) {
+                            const float f = s_o[c * kKv4MaxRuns + i + u * SUB];
+                            O = make_float2(fmaf(ahead[u].x, f, O.x), fmaf(ahead[u].y, f, O.y));
+                        }
                 }
+                if (SUB == 1)
+                    kv4_put<HD>(a, it, g, c, e % (HD / 2) * 2, O, s_l[c][0]);
+                else
+                    s_red[sub * pairs + e] = O;
+            }
+            if (SUB > 1) {
                 __syncthreads();
-                bool fresh = true;
-                for (int e = e0; busy && e < pairs; e += NT) {
-                    const int c = e / (HD / 2);
-                    float2 O = make_float2(0.f, 0.f);
-                    for (int i = sub; i < parts; i += AHEAD * SUB) {
-                        if (!fresh) grab(e, i);
-                        fresh = false;
-#pragma unroll
-                        for (int u = 0; u < AHEAD; u++)
-                            if (i + u * SUB < parts) {
-                                const float f = s_o[c * kKv4MaxRuns + i + u * SUB];
-                                O = make_float2(fmaf(ahead[u].x, f, O.x), fmaf(ahead[u].y, f, O.y));
-                            }
-                    }
-                    if (SUB == 1)
-                        kv4_put<HD>(a, it, g, c, e % (HD / 2) * 2, O, s_l[c][0]);
-                    else
-                        s_red[sub * pairs + e] = O;
-                }
-                if (SUB > 1) {
-                    __syncthreads();
-                    if (t < pairs) {
-                        float2 O = s_red[t];
-                        for (int i = 1; i < SUB; i++) O = make_float2(O.x + s_red[i * pairs + t].x, O.y + s_red[i * pairs + t].y);
-                        kv4_put<HD>(a, it, g, t / (HD / 2), t % (HD / 2) * 2, O, s_l[t / (HD / 2)][0]);
-                    }
+                if (t < pairs) {
+                    float2 O = s_red[t];
+                    for (int i = 1; i < SUB; i++) O = make_float2(O.x + s_red[i * pairs + t].x, O.y + s_red[i * pairs + t].y);
+                    kv4_put<HD>(a, it, g, t / (HD / 2), t % (HD / 2) * 2, O, s_l[t / (HD / 2)][0]);
                 }
             }
         }
-        __syncthreads();
-        it = it_next;
     }
 }
 
@@ -1185,7 +1163,7 @@ Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq) {
     const int tc = 64 * kColTiles;
     p.ntile = (int)((ncol + tc - 1) / tc);
     p.items = (int64_t)p.ntile * c.n_seq;
-    p.runs = 1;
+    p.runs = 1;  // (of the tile kernel)
     p.tile = ncol > kKv4RowCols && p.items * c.nkv >= kKv4TileWorkgroups;
     if (p.tile) return p;
     p.part_cols = (int)std::min<int64_t>(16, ncol);
@@ -1195,18 +1173,17 @@ Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq) {
     const int block = one && c.hd < 256 ? 32 * kv4_waves<128, true>() : 32 * kv4_waves<128, false>();
     const int64_t nb = ((int64_t)c.cap + block - 1) / block;
     const int groups = one && c.hd < 256 ? kKv4Workgroups / 2 : kKv4Workgroups;
-    p.flat = !one && p.items * c.nkv <= kKv4Workgroups && p.items * nb <= 1 << 30;
-    if (one || p.flat) {
-        p.runs = (int)std::min<int64_t>({kKv4MaxRuns, p.items * nb, std::max(1, groups / c.nkv)});
-        p.split = nb > 1 && p.runs > 1;
-    } else {
-        p.runs = (int)std::min<int64_t>(p.items, 0x7fffffff);
-    }
+    const int64_t most = std::min<int64_t>(p.items * nb, std::max(1, groups / c.nkv));
+    // (kv4_deal counts up to 2^21 blocks)
+    const bool share = c.cap > kKv4WholeKeys && most > 1;
+    p.flat = share && !one && p.items * c.nkv <= kKv4Workgroups && nb <= 1 << 20;
+    p.split = share && (one || p.flat);
+    p.runs = (int)(!p.split ? p.items : one ? std::min<int64_t>(most, kKv4MaxRuns) : most);
     return p;
 }
 
-// Partial states of a launch: a run has two slots.
-static size_t kv4_part_states(const Kv4Plan &p, int nkv) { return p.split ? (size_t)2 * nkv * p.runs * p.part_cols : 0; }
+// Partial states of a launch.
+static size_t kv4_part_states(const Kv4Plan &p, int nkv) { return p.split ? (size_t)nkv * p.runs * p.part_cols : 0; }
 
 size_t kv4_attn_ws_bytes(const Kv4Cache &c, int rows, int nq) {
     const size_t n = kv4_part_states(plan_kv4_attn(c, rows, nq), c.nkv);

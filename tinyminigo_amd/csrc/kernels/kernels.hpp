@@ -408,10 +408,10 @@ struct Kv4AttnArgs {
     // rows to append first ([nkv][hd], new_stride floats apart), or null
     const float *k_new, *v_new;
     size_t new_stride;
-    // set by launch_kv4_attn (see Kv4Plan): the runs' partial states [KV
-    // head][run][2][part_cols] of hd floats in part and of (max, sum) in
-    // part_ml, and per KV head and run the count of the arrived parts of the
-    // shared item that starts in it
+    // set by launch_kv4_attn (see Kv4Plan): the workgroups' partial states [KV
+    // head][run][part_cols] of hd floats in part and of (max, sum) in part_ml,
+    // and per KV head and run the count of the arrived parts of the item whose
+    // first workgroup it is
     int group, ntile, items, flat, runs, part_cols;
     float inv_group;  // 1 / group
     unsigned *arrived;
@@ -419,10 +419,10 @@ struct Kv4AttnArgs {
 };
 constexpr int kKv4Workgroups = 512;   // of 256 threads: two per CU
 constexpr int kKv4MaxRuns = 256;
-// Most items cut into equal runs: more of them, times the KV heads, than
-// kKv4Workgroups are a workgroup each.
+// Most items that workgroups are shared out to: more of them, times the KV
+// heads, than kKv4Workgroups are a workgroup each.
 constexpr int kKv4FlatItems = kKv4Workgroups;
-constexpr int kKv4WholeBlocks = 2;    // blocks that one workgroup takes rather than share
+constexpr int kKv4WholeKeys = 512;    // positions that one workgroup takes rather than share
 // Counters of the shared items, one a workgroup at most, at the start of the
 // workspace.
 constexpr size_t kKv4CounterBytes = kKv4Workgroups * 4;
@@ -439,12 +439,12 @@ struct Kv4Plan {
     int ntile;      // column tiles of a sequence
     int64_t items;  // column tiles of all sequences
     int runs;       // rows kernel: workgroups of a KV head
-    bool flat;      // rows kernel: the items' blocks are cut into equal runs
+    bool flat;      // rows kernel: several items, an item's blocks may be shared
     bool split;     // rows kernel: an item may be shared by several workgroups
 };
 Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq);
 // Workspace bytes that no call of this head dim exceeds.
-constexpr size_t kv4_attn_most_ws_bytes(int hd) { return kKv4CounterBytes + (size_t)2 * kKv4Workgroups * 16 * (hd + 2) * 4; }
+constexpr size_t kv4_attn_most_ws_bytes(int hd) { return kKv4CounterBytes + (size_t)kKv4Workgroups * 16 * (hd + 2) * 4; }
 // Workspace enough for every position: counters, which are zero between
 // launches, then the partial states.
 size_t kv4_attn_ws_bytes(const Kv4Cache &c, int rows, int nq);

@@ -309,6 +309,46 @@ def test_attn_long_prompt(T, H):
         check_attn(c, got[:, t:t + 1], q[:, t:t + 1], [71 + t])
 
 
+def test_attn_longer_prompt(T, H):
+    """Enough rows of one sequence for the prompts' kernel."""
+    rng = np.random.default_rng(78)
+    c = Cache(T, H, 3021, 8, 128)
+    c.fill(rng, 3021)
+    q = rng.standard_normal((1, 3000, 16, 128)).astype(np.float32)
+    got = attend(c, q, [21])
+    for t in (0, 1, 63, 64, 1000, 2047, 2999):
+        check_attn(c, got[:, t:t + 1], q[:, t:t + 1], [21 + t])
+
+
+@pytest.mark.parametrize("hd,group,n", [(32, 2, 17), (64, 4, 9), (128, 2, 32), (256, 3, 11)])
+def test_attn_prompts_of_one_tile(T, H, hd, group, n):
+    """More sequences, each of one tile of columns."""
+    rng = np.random.default_rng(hd + group + n)
+    c = Cache(T, H, n + 100, 4, hd, n_seq=180)
+    c.fill(rng, n + 100)
+    pos = [int(x) for x in rng.integers(0, 100, 180)]
+    pos[0], pos[1], pos[2], pos[3] = 0, 100, -1, 101
+    q = rng.standard_normal((180, n, 4 * group, hd)).astype(np.float32)
+    check_attn(c, attend(c, q, pos, dev=ints(H, pos)), q, pos, only=(0, 1, 2, 3, 90, 179))
+
+
+@pytest.mark.parametrize("n_seq,nkv,group,cap", [(2, 4, 2, 3000), (63, 2, 2, 1600), (64, 8, 1, 900), (65, 1, 4, 2500),
+                                                 (130, 1, 2, 1500), (256, 2, 3, 700), (512, 1, 2, 700), (513, 1, 2, 600)])
+def test_attn_of_many_ragged_sequences(T, H, n_seq, nkv, group, cap):
+    """A few long sequences among short ones and idle slots, up to as many as
+    share a launch's workgroups, and one more."""
+    rng = np.random.default_rng(n_seq)
+    c = Cache(T, H, cap, nkv, 16, n_seq=n_seq)
+    c.fill(rng, cap)
+    pos = rng.integers(0, 40, n_seq)
+    pos[rng.integers(0, n_seq, max(2, n_seq // 4))] = rng.integers(cap // 2, cap, max(2, n_seq // 4))
+    pos[rng.integers(0, n_seq, n_seq // 9)] = -1
+    pos[0], pos[-1] = cap - 1, rng.integers(0, cap)
+    pos = [int(p) for p in pos]
+    q = rng.standard_normal((n_seq, 1, nkv * group, 16)).astype(np.float32)
+    check_attn(c, attend(c, q, pos, dev=ints(H, pos)), q, pos)
+
+
 @pytest.mark.parametrize("hd", [16, 32, 64, 128, 256])
 def test_attn_prompts_with_values_of_all_sizes(T, H, hd):
     """Sequences of values around 1, growing by 2^60 within a block of keys and

@@ -548,7 +548,7 @@ __device__ __forceinline__ float uniform(float v) {
 // all of them come to the same numbers.  False where workgroup `run` has none.
 template <int BLOCK>
 __device__ __forceinline__ bool kv4_deal(const Kv4AttnArgs &a, int run, int lane, int *item, int *part, int *parts) {
-    constexpr int PER = kKv4FlatItems / 64;  // items of a lane: 64 i + lane
+    constexpr int PER = kKv4DealItems / 64;  // items of a lane: 64 i + lane
     float n[PER], total = 0.f, most = 1.f;   // (integers below 2^24)
 #pragma unroll
     for (int i = 0; i < PER; i++) {
@@ -634,7 +634,7 @@ constexpr int kv4_waves() {
 // - ONE item: a workgroup's first block does not hang on the position, so its
 //   keys are loaded before the position, which may live on the device, is
 //   known.
-// - Up to kKv4FlatItems items (a.flat): kv4_deal shares the workgroups out.
+// - Up to kKv4DealItems items (a.deal): kv4_deal shares the workgroups out.
 //   (The same number of them for every item left sequences of 65 to 131070
 //   positions at 100 us, 1.9 times the time of their mean.)
 // - More items: a workgroup each.
@@ -721,7 +721,7 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
 
     int pos0 = a.pos;
     int item = 0, part = 0, parts = 1;  // this workgroup's, and those that share the item
-    const bool flat = !ONE && a.flat;
+    const bool deal = !ONE && a.deal;
     if constexpr (ONE) {
         // the query first: it is split while the first keys are on their way
         fetch(0, 0, 0, min(16, a.rows * a.group));
@@ -734,7 +734,7 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
             for (int h = 0; h < Kv4Query<HD, C>::KH; h++)
 #pragma unroll
                 for (int set = 0; set < Kv4Lanes<C>::QSETS; set++) asm volatile("" : "+v"(q.part[h][set]));
-    } else if (flat) {
+    } else if (deal) {
         if (!kv4_deal<BLOCK>(a, run, lane, &item, &part, &parts)) return;
     } else {
         item = a.items - 1 - run;  // the latest rows, with the most keys, first
@@ -1176,8 +1176,8 @@ Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq) {
     const int64_t most = std::min<int64_t>(p.items * nb, std::max(1, groups / c.nkv));
     // (kv4_deal counts up to 2^21 blocks)
     const bool share = c.cap > kKv4WholeKeys && most > 1;
-    p.flat = share && !one && p.items * c.nkv <= kKv4Workgroups && nb <= 1 << 20;
-    p.split = share && (one || p.flat);
+    p.deal = share && !one && p.items * c.nkv <= kKv4Workgroups && nb <= 1 << 20;
+    p.split = share && (one || p.deal);
     p.runs = (int)(!p.split ? p.items : one ? std::min<int64_t>(most, kKv4MaxRuns) : most);
     return p;
 }
@@ -1231,7 +1231,7 @@ hipError_t launch_kv4_attn(Kv4AttnArgs a, void *ws, hipStream_t s) {
     a.inv_group = 1.0f / (float)a.group;
     a.ntile = p.ntile;
     a.items = (int)p.items;
-    a.flat = p.flat;
+    a.deal = p.deal;
     a.runs = p.runs;
     a.part_cols = p.part_cols;
     a.arrived = (unsigned *)ws;

@@ -412,7 +412,7 @@ struct Kv4AttnArgs {
     // head][run][part_cols] of hd floats in part and of (max, sum) in part_ml,
     // and per KV head and run the count of the arrived parts of the item whose
     // first workgroup it is
-    int group, ntile, items, flat, runs, part_cols;
+    int group, ntile, items, deal, runs, part_cols;
     float inv_group;  // 1 / group
     unsigned *arrived;
     float *part, *part_ml;
@@ -420,26 +420,36 @@ struct Kv4AttnArgs {
 constexpr int kKv4Workgroups = 512;   // of 256 threads: two per CU
 constexpr int kKv4MaxRuns = 256;
 // Most items that workgroups are shared out to: more of them, times the KV
-// heads, than kKv4Workgroups are a workgroup each.
-constexpr int kKv4FlatItems = kKv4Workgroups;
-constexpr int kKv4WholeKeys = 512;    // positions that one workgroup takes rather than share
+// heads, than kKv4Workgroups are a workgroup each.  (As many workgroups as run
+// at a time: with twice as many to share out, 48 sequences of 2001 positions
+// take 33 us instead of 25.)
+constexpr int kKv4DealItems = kKv4Workgroups;
+// Positions that one workgroup takes rather than share: with 256 instead, 400
+// tokens take 16.0 us instead of 10.0 and 32 sequences of 301 positions 11.8
+// instead of 11.1, with 1024 8 of 2001 take 14.2 instead of 11.4.
+constexpr int kKv4WholeKeys = 512;
 // Counters of the shared items, one a workgroup at most, at the start of the
 // workspace.
 constexpr size_t kKv4CounterBytes = kKv4Workgroups * 4;
 // More columns (query rows x heads of a KV head) of a sequence than kKv4RowCols
 // take the tile kernel, where its tiles are kKv4TileWorkgroups workgroups or
-// more: 16 heads over 8 of 128, 1000 / 2000 / 4000 tokens (256 / 504 / 1000
-// tiles) 40 / 74 / 155 us against the rows kernel's 30 / 73 / 208, 2000 tokens
-// after 6000 283 against 314.
+// more.  Times with the tile kernel against the rows kernel, us:
+//   16 heads over 8 of 128, 1000 / 2500 / 3500 / 4500 tokens (256 / 632 / 880 /
+//   1128 tiles) 41 / 96 / 136 / 184 against 25 / 84 / 148 / 231, 2000 and 2500
+//   after 6000 287 and 349 against 290 and 373;
+//   32 over 8 of 128, 1000 / 1500 / 2500 (504 / 752 / 1256) 44 / 65 / 131
+//   against 39 / 72 / 163;
+//   head dim 64, 2000 / 3000 (500 / 750) 59 / 88 against 49 / 94; 256, 4000 /
+//   6000 (500 / 752) 297 / 460 against 255 / 516.
 constexpr int kKv4RowCols = 32;
-constexpr int64_t kKv4TileWorkgroups = 500;
+constexpr int64_t kKv4TileWorkgroups = 700;
 struct Kv4Plan {
     bool tile;      // the tile kernel, else the rows kernel
     int part_cols;  // columns of an item's partial states
     int ntile;      // column tiles of a sequence
     int64_t items;  // column tiles of all sequences
     int runs;       // rows kernel: workgroups of a KV head
-    bool flat;      // rows kernel: several items, an item's blocks may be shared
+    bool deal;      // rows kernel: several items, an item's blocks may be shared
     bool split;     // rows kernel: an item may be shared by several workgroups
 };
 Kv4Plan plan_kv4_attn(const Kv4Cache &c, int rows, int nq);

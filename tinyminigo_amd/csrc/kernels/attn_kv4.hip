@@ -616,9 +616,11 @@ __device__ __forceinline__ void kv4_put(const Kv4AttnArgs &a, const Kv4Item &it,
 }
 
 // Wavefronts of a workgroup; a wavefront takes 32 keys of a block.  One item
-// alone is spread over eight (fewer workgroups to merge); of several, two
-// workgroups of four share a CU, so that one's loads, query and merge run
-// beside the other's products (48 ragged sequences: 44 us with one of eight).
+// alone is spread over eight (fewer workgroups to merge: at 8300 positions 11.2
+// us against 12.4 with four, at 200 5.7 against 5.3); of several, two workgroups
+// of four share a CU, so that one's loads, query and merge run beside the
+// other's products (64 sequences of 2001 positions 26.7 us against 29.0 with
+// one of eight, 500 tokens 11.1 against 15.4; 32 of 2001 20.5 against 16.2).
 // At head dim 256 the registers leave room for one wavefront a SIMD.
 template <int HD, bool ONE>
 constexpr int kv4_waves() {
@@ -642,8 +644,11 @@ constexpr int kv4_waves() {
 // With a.k_new (one row a sequence) the wavefront that owns the new position
 // quantizes the row, stores it and takes it from LDS; no other needs it.
 //
-// Bound by the latency of its loads and of the merge for one sequence, by the
-// cache's bytes for many.
+// Bound by the latency of its loads and of the merge for one sequence (16 heads
+// over 8 of 128: 6.0 us at 320 positions, 11 at 8300) or a few (14 of up to 1003
+// positions 11 us); by VALU issue (78%: a value takes a conversion and half a
+// permute) and the cache's bytes for many: four sequences, 271 thousand
+// positions, 56.6 us, 5.2 TB/s.
 template <int HD, bool ONE, int C>
 __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) void kv4_attn_rows_kernel(const Kv4AttnArgs a) {
     constexpr int DPL = HD / 16, PITCH = HD + 4, NW = kv4_waves<HD, ONE>(), NT = 64 * NW, BLOCK = 32 * NW;
@@ -998,7 +1003,10 @@ struct Kv4Stage {
 // lane's operand is 16 bytes at 16 lane: no bank conflicts), a block ahead.
 //
 // Workgroups of the latest positions come first: they have the most keys.
-// Bound by the MFMA and VALU issue of its three wavefronts a SIMD.
+// Bound by the issue of its three wavefronts a SIMD (MFMA busy 49%, VALU 66%):
+// 8192 tokens, 16 heads over 8 of 128, 546-566 us, 486-503 TFLOP/s of the
+// causal products' 275 GFLOP; with the parts of Q and P the matrix cores do
+// 2.25 times that.
 template <int HD>
 __global__ __launch_bounds__(kBlock, HD == 256 ? 2 : 3) void kv4_attn_tile_kernel(const Kv4AttnArgs a) {
     constexpr int DPL = HD / 16, CT = kColTiles, TC = 64 * CT;

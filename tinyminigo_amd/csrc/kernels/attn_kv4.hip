@@ -546,17 +546,19 @@ __device__ __forceinline__ float uniform(float v) {
 // can be) for which there are enough, so every workgroup has one item and most
 // have as many blocks.  Every wavefront finds its workgroup's share by itself;
 // all of them come to the same numbers.  False where workgroup `run` has none.
+// blocks: kKv4DealItems floats in LDS, to which all wavefronts write the same.
 template <int BLOCK>
-__device__ __forceinline__ bool kv4_deal(const Kv4AttnArgs &a, int run, int lane, int *item, int *part, int *parts) {
-    constexpr int PER = kKv4DealItems / 64;  // items of a lane: 64 i + lane
-    float n[PER], total = 0.f, most = 1.f;   // (integers below 2^24)
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        if (64 * i >= a.items) continue;
-        n[i] = 64 * i + lane < a.items ? (float)max(1, kv4_item<BLOCK>(a, 64 * i + lane).nb) : 0.f;
-        total += n[i];
-        most = fmaxf(most, n[i]);
+__device__ __forceinline__ bool kv4_deal(const Kv4AttnArgs &a, int run, int lane, float *blocks, int *item, int *part, int *parts) {
+    float total = 0.f, most = 1.f;  // (integers below 2^24)
+#pragma unroll 1
+    for (int i = lane; i < a.items; i += 64) {
+        const float n = (float)max(1, kv4_item<BLOCK>(a, i).nb);
+        blocks[i] = n;
+        total += n;
+        most = fmaxf(most, n);
     }
+    // a lane reads what it wrote itself
+    const float n0 = lane < a.items ? blocks[lane] : 0.f;
     total = uniform(wave_sum(total));
     most = uniform(wave_max(most));
     float inv = 0.f;  // 1 / each
@@ -568,19 +570,17 @@ __device__ __forceinline__ bool kv4_deal(const Kv4AttnArgs &a, int run, int lane
     for (int turn = 0; turn < 5 && lo < hi; turn++) {
         const int mid = (lo + hi) >> 1;
         inv = __builtin_amdgcn_rcpf((float)mid);
-        int sum = 0;
-#pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (64 * i < a.items) sum += share(n[i]);
+        int sum = share(n0);
+#pragma unroll 1
+        for (int i = lane + 64; i < a.items; i += 64) sum += share(blocks[i]);
         if ((int)uniform(wave_sum((float)sum)) <= a.runs) hi = mid;
         else lo = mid + 1;
     }
     inv = __builtin_amdgcn_rcpf((float)hi);
     int before = 0;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        if (64 * i >= a.items) continue;
-        const int mine = share(n[i]);
+#pragma unroll 1
+    for (int i = 0; i < a.items; i += 64) {
+        const int mine = share(i == 0 ? n0 : i + lane < a.items ? blocks[i + lane] : 0.f);
         int upto = mine;  // over the lanes up to this one
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -591,7 +591,7 @@ __device__ __forceinline__ bool kv4_deal(const Kv4AttnArgs &a, int run, int lane
         const unsigned long long here = __builtin_amdgcn_ballot_w64(run >= first && run < first + mine);
         if (here) {
             const int l = __builtin_ctzll(here);
-            *item = 64 * i + l;
+            *item = i + l;
             *part = run - __builtin_amdgcn_readlane(first, l);
             *parts = __builtin_amdgcn_readlane(mine, l);
             return true;
@@ -659,6 +659,7 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
     __shared__ Kv4SharedQuery<C == 16 ? HD : 16> s_q;
     __shared__ Kv4NewRow<HD> s_new;
     __shared__ unsigned s_arrived;
+    __shared__ float s_blocks[ONE ? 1 : kKv4DealItems];
     __shared__ float2 s_red[NT];
     const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, r = lane & 15, lg = lane >> 4;
     // (run, KV head): one item's runs read different keys; several items' tiles
@@ -740,7 +741,7 @@ __global__ __launch_bounds__((64 * kv4_waves<HD, ONE>()), (HD == 256 ? 1 : 2)) v
 #pragma unroll
                 for (int set = 0; set < Kv4Lanes<C>::QSETS; set++) asm volatile("" : "+v"(q.part[h][set]));
     } else if (deal) {
-        if (!kv4_deal<BLOCK>(a, run, lane, &item, &part, &parts)) return;
+        if (!kv4_deal<BLOCK>(a, run, lane, s_blocks, &item, &part, &parts)) return;
     } else {
         item = a.items - 1 - run;  // the latest rows, with the most keys, first
     }

@@ -420,6 +420,31 @@ def test_attn_appends_rows(T, H, n, hd):
         check_attn(c, got, q, pos)
 
 
+@pytest.mark.parametrize("n_seq", [1, 4])
+@pytest.mark.parametrize("n,group", [(1, 2), (1, 3), (1, 20), (5, 2)])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128, 256])
+def test_attn_appends_rows_to_shared_sequences(T, H, n_seq, n, group, hd):
+    """Positions of which several workgroups take a part, and the step from one
+    workgroup to several; marked groups of values and keys among them."""
+    rng = np.random.default_rng(n + hd + group)
+    c = Cache(T, H, 1500, 2, hd, n_seq=n_seq)
+
+    def spoil(x, at):
+        x[n_seq - 1, at, 1, hd // 2] = np.inf
+        return x
+    c.fill(rng, 1480, keys=lambda k: spoil(k, 1300), values=lambda v: spoil(v, 700))
+    at = [1470, 510, -1, 1280][:n_seq]
+    for step in range(4):
+        pos = [p + step * n if p >= 0 else p for p in at]
+        new = rows(rng, c, n), rows(rng, c, n)
+        if step == 2:
+            new[1][0, 0, 0, 3] = np.nan
+        q = rng.standard_normal((n_seq, n, 2 * group, hd)).astype(np.float32)
+        got = attend(c, q, pos, dev=ints(H, pos), new=new)
+        c.check()
+        check_attn(c, got, q, pos)
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_attn_append_idle_slots_write_nothing(T, H, n):
     rng = np.random.default_rng(n)
@@ -564,6 +589,38 @@ def test_attn_on_a_stream_and_in_graphs(T, H):
             np.testing.assert_array_equal(got, eager)
             check_attn(c, got, q[i], pos)
         c.check()
+
+
+@pytest.mark.parametrize("n_seq", [1, 3])
+def test_shared_sequences_in_graphs(T, H, n_seq):
+    """Two graphs with one workspace whose sequences grow from one workgroup to
+    several, an eager call between the replays."""
+    rng = np.random.default_rng(80 + n_seq)
+    c = Cache(T, H, 1600, 2, 128, n_seq=n_seq)
+    c.fill(rng, 1600)
+    nq, s = 4, H.Stream()
+    size = n_seq * nq * 128
+    qd, out = ([H.DeviceBuffer(size * 4) for _ in range(2)] for _ in range(2))
+    pd = ints(H, [0] * n_seq)
+    ws = H.DeviceBuffer(T.kv4_attn_workspace(c.kv, 1, nq))
+    ws.fill_byte(0)
+
+    def step(i):
+        return lambda st: T.kv4_attn(c.kv, qd[i].addr, out[i].addr, 1, nq, pos_dev=pd.addr, ws_dev=ws.addr,
+                                     ws_bytes=ws.nbytes, stream=st.addr)
+    graphs = [H.Graph(s, step(i)) for i in range(2)]
+    for first in (510, 511, 512, 1599, 700, 1100):
+        pos = [first, 900, 20][:n_seq]
+        q = rng.standard_normal((2, n_seq, 1, nq, 128)).astype(np.float32)
+        for d, x in [(qd[0], q[0]), (qd[1], q[1]), (pd, np.asarray(pos, np.int32))]:
+            H.copy_device(d, H.DeviceBuffer.from_array(x), x.nbytes)
+        for g in graphs:
+            g.launch()
+        s.synchronize()
+        for i in range(2):
+            got = out[i].to_array(np.float32, size).reshape(q[i].shape)
+            np.testing.assert_array_equal(got, attend(c, q[i], pos, dev=ints(H, pos)))
+            check_attn(c, got, q[i], pos)
 
 
 def test_attn_two_streams_at_once(T, H):

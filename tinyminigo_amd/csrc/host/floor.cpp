@@ -139,8 +139,8 @@ extern "C" int tmg_profile_step_floor(tmg_model *m, tmg_cache *c, uint32_t token
     if (n_records) *n_records = 0;
     if (!m || !c || c->model != m) return set_error(TMG_E_INVALID, "bad model/cache handle");
     if (token >= (uint32_t)m->V) return set_error(TMG_E_INVALID, "token id out of range");
-    // every replay of the step advances the position by one
     if (c->kv4) return set_error(TMG_E_INVALID, "the step floor is that of f32 caches");
+    // every replay of the step advances the position by one
     if ((size_t)c->len + kReps + 1 >= c->max_pos) return set_error(TMG_E_CAPACITY, "KV cache too short for the replays");
     (void)hipSetDevice(m->device);
     int rc;

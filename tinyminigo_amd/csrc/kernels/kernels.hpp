@@ -426,7 +426,10 @@ constexpr int kKv4MaxRuns = 256;
 constexpr int kKv4DealItems = kKv4Workgroups;
 // Positions that one workgroup takes rather than share: with 256 instead, 400
 // tokens take 16.0 us instead of 10.0 and 32 sequences of 301 positions 11.8
-// instead of 11.1, with 1024 8 of 2001 take 14.2 instead of 11.4.
+// instead of 11.1, with 1024 8 of 2001 take 14.2 instead of 11.4.  It is the
+// least share of what is shared as well: with 384 for that, 45 tokens after 1630
+// take 15.2 us instead of 15.7 and 8 sequences of 2001 12.2 instead of 11.1;
+// with 128, 16 tokens after 3000 take 23.1 instead of 15.8.
 constexpr int kKv4WholeKeys = 512;
 // Counters of the shared items, one a workgroup at most, at the start of the
 // workspace.

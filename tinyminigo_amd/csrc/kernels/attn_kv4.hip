@@ -1005,9 +1005,10 @@ struct Kv4Stage {
 //
 // Workgroups of the latest positions come first: they have the most keys.
 // Bound by the issue of its three wavefronts a SIMD (MFMA busy 49%, VALU 66%):
-// 8192 tokens, 16 heads over 8 of 128, 546-566 us, 486-503 TFLOP/s of the
-// causal products' 275 GFLOP; with the parts of Q and P the matrix cores do
-// 2.25 times that.
+// 8192 tokens, 16 heads over 8 of 128, 546-567 us, 485-503 TFLOP/s of the
+// causal products' 275 GFLOP.  With the parts of Q and P that is 618 GFLOP in
+// bf16 products' time: 1.09-1.13 PFLOP/s, where a plain bf16 product of 8192^3
+// reaches 1.19.  (Wave priorities around the products or the softmax: 567-571.)
 template <int HD>
 __global__ __launch_bounds__(kBlock, HD == 256 ? 2 : 3) void kv4_attn_tile_kernel(const Kv4AttnArgs a) {
     constexpr int DPL = HD / 16, CT = kColTiles, TC = 64 * CT;
